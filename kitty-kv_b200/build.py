@@ -1,11 +1,12 @@
-"""Build the Kitty B200 CUDA library in-tree.
+"""Build the Kitty B200 CUDA libraries in-tree.
 
-    python kitty-kv_b200/build.py            # -> kitty-kv_b200/kitty/libkitty_b200.so
+    python kitty-kv_b200/build.py            # -> kitty-kv_b200/kitty/libkitty_b200.so, libkitty_kv8.so
 
 Compiles every ``csrc/*.cu`` for sm_100a only (no PTX for other targets) with
 IEEE float32 division and square root (no --use_fast_math: the quantisers must
 round exactly like the reference) and links one shared library exporting the
-C ABI declared in ``include/kitty_b200.h``.  Objects go to ``_build/``.
+C ABI declared in ``include/kitty_b200.h``; ``csrc/kv8/*.cu`` (the 8-bit cache) make
+a second one with the C ABI of ``include/kitty_kv8.h``.  Objects go to ``_build/``.
 """
 
 from __future__ import annotations
@@ -14,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_ROOT = Path(__file__).resolve().parent
@@ -21,6 +23,7 @@ REPO_ROOT = PKG_ROOT.parent
 CSRC = PKG_ROOT / "csrc"
 BUILD = PKG_ROOT / "_build"
 LIB = PKG_ROOT / "kitty" / "libkitty_b200.so"
+LIB_KV8 = PKG_ROOT / "kitty" / "libkitty_kv8.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -35,28 +38,36 @@ def nvcc() -> str:
 
 
 def build(verbose: bool = False, extra: list | None = None) -> Path:
+    headers = [*CSRC.glob("*.cuh"), REPO_ROOT / "include" / "kitty_b200.h"]
+    _library(LIB, CSRC.glob("*.cu"), headers, [], verbose, extra)
+    headers = [*(CSRC / "kv8").glob("*.cuh"), *(REPO_ROOT / "include").glob("*.h")]
+    _library(LIB_KV8, (CSRC / "kv8").glob("*.cu"), headers, ["-Xcompiler", "-fvisibility=hidden"], verbose, extra)
+    return LIB
+
+
+def _library(lib: Path, sources, headers, flags: list, verbose: bool, extra: list | None) -> None:
+    """Compile what is older than its source or the headers (sources side by side) and link."""
     BUILD.mkdir(exist_ok=True)
-    sources = sorted(CSRC.glob("*.cu"))
-    headers = sorted(CSRC.glob("*.cuh")) + [REPO_ROOT / "include" / "kitty_b200.h"]
     newest_header = max(h.stat().st_mtime for h in headers)
-    objs = []
-    for src in sources:
+    objs, cmds = [], []
+    for src in sorted(sources):
         obj = BUILD / (src.stem + ".o")
         objs.append(obj)
         if obj.exists() and obj.stat().st_mtime >= max(src.stat().st_mtime, newest_header):
             continue
-        cmd = [nvcc(), *ARCH, *NVCC_FLAGS, *(extra or []), "-c", str(src), "-o", str(obj)]
+        cmds.append([nvcc(), *ARCH, *NVCC_FLAGS, *flags, *(extra or []), "-c", str(src), "-o", str(obj)])
         if verbose:
-            print(" ".join(cmd), flush=True)
-        subprocess.run(cmd, check=True)
-    if (not LIB.exists()) or any(o.stat().st_mtime > LIB.stat().st_mtime for o in objs):
-        tmp = LIB.with_suffix(".so.tmp")
+            print(" ".join(cmds[-1]), flush=True)
+    with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+        for done in [pool.submit(subprocess.run, cmd, check=True) for cmd in cmds]:
+            done.result()
+    if (not lib.exists()) or any(o.stat().st_mtime > lib.stat().st_mtime for o in objs):
+        tmp = lib.with_suffix(".so.tmp")
         cmd = [nvcc(), *ARCH, "-shared", "-cudart", "static", "-o", str(tmp), *map(str, objs)]
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
-        os.replace(tmp, LIB)
-    return LIB
+        os.replace(tmp, lib)
 
 
 if __name__ == "__main__":

@@ -1,0 +1,191 @@
+// RMS norm of every query and key head with the rotary embedding in the same pass.
+//
+// A row (one head of one token, D channels) is held by the lanes of a group: the lane
+// that rotates pairs 8j .. 8j+7 has all sixteen values of those pairs in registers
+// (two 16-byte loads), so the rotation needs no exchange and the mean of squares one
+// butterfly over the group.  A warp keeps its token's cosines and sines over up to
+// kPasses rows per group and issues the loads of all of them first.
+#include "kv8_common.cuh"
+
+namespace kitty8 {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kPasses = 4;     // rows per lane group and token: the table values are read once for them
+
+struct RopeShape {
+  int q_chunks, chunks;        // warps per token: ceil(heads / rows of a warp), queries first
+};
+
+template <bool kBf16, int kLanes, bool kInter>
+__global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(KittyQkNormRopeArgs a, RopeShape sh, uint32_t* err) {
+  constexpr int kRows = 32 / kLanes;                       // rows that a warp holds at once
+  const int lane = threadIdx.x & 31, j = lane % kLanes;
+  const int64_t warps = int64_t(gridDim.x) * (kThreads / 32) / sh.chunks * sh.chunks;
+  const int64_t gw = int64_t(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  if (gw >= warps) return;
+  const int chunk = int(gw % sh.chunks);                   // the same heads for every token of this warp
+  const bool is_q = chunk < sh.q_chunks;
+  const int heads = is_q ? a.num_q_heads : a.num_k_heads;
+  const int h0 = (is_q ? chunk : chunk - sh.q_chunks) * (kRows * kPasses) + lane / kLanes;
+  const int D = a.head_dim, pair_lanes = a.rot / 16;
+  const bool active = j < D / 16, rotates = j < pair_lanes;
+  // first channel of the lane's two groups of eight
+  int c0, c1;
+  if (kInter || !rotates) {
+    c0 = rotates ? 16 * j : a.rot + 16 * (j - pair_lanes);
+    c1 = c0 + 8;
+  } else {
+    c0 = 8 * j;
+    c1 = c0 + a.rot / 2;
+  }
+  const uint16_t* in = static_cast<const uint16_t*>(is_q ? a.q : a.k);
+  uint16_t* out = static_cast<uint16_t*>(is_q ? a.q_out : a.k_out);
+  const int64_t s_row = is_q ? a.q_s_row : a.k_s_row, s_head = is_q ? a.q_s_head : a.k_s_head;
+  const int64_t o_row = is_q ? a.qo_s_row : a.ko_s_row, o_head = is_q ? a.qo_s_head : a.ko_s_head;
+  const void* wp = is_q ? a.q_weight : a.k_weight;
+  float w[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int c = (i < 8 ? c0 : c1 - 8) + i;
+    w[i] = 1.f;
+    if (wp && active) {
+      if (a.weight_f32) w[i] = static_cast<const float*>(wp)[c];
+      else w[i] = dev::to_f2<kBf16>(static_cast<const uint16_t*>(wp)[c]).x;
+    }
+  }
+  const float inv_d = 1.f / float(D);
+  for (int64_t t = gw / sh.chunks; t < a.rows; t += warps / sh.chunks) {
+    const int64_t pos = a.positions64 ? static_cast<const int64_t*>(a.positions)[t]
+                                      : int64_t(static_cast<const int32_t*>(a.positions)[t]);
+    if (pos < 0) continue;                                  // a padding row
+    if (pos >= a.table_rows) {
+      if (lane == 0) dev::flag(err, kErrPosition);
+      continue;
+    }
+    uint4 x[kPasses][2];
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int h = h0 + p * kRows;
+      if (active && h < heads) {
+        const uint16_t* r = in + t * s_row + h * s_head;
+        x[p][0] = *reinterpret_cast<const uint4*>(r + c0);
+        x[p][1] = *reinterpret_cast<const uint4*>(r + c1);
+      } else {
+        x[p][0] = x[p][1] = make_uint4(0, 0, 0, 0);
+      }
+    }
+    float cs[8], sn[8];
+    if (rotates) {
+      const float4* tc = reinterpret_cast<const float4*>(a.table + pos * a.rot + 8 * j);
+      const float4* ts = reinterpret_cast<const float4*>(a.table + pos * a.rot + a.rot / 2 + 8 * j);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float4 u = __ldg(tc + i), v = __ldg(ts + i);
+        cs[4 * i] = u.x; cs[4 * i + 1] = u.y; cs[4 * i + 2] = u.z; cs[4 * i + 3] = u.w;
+        sn[4 * i] = v.x; sn[4 * i + 1] = v.y; sn[4 * i + 2] = v.z; sn[4 * i + 3] = v.w;
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int h = h0 + p * kRows;
+      float y[16];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t u[4] = {x[p][half].x, x[p][half].y, x[p][half].z, x[p][half].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = dev::to_f2<kBf16>(u[i]);
+          y[8 * half + 2 * i] = f.x;
+          y[8 * half + 2 * i + 1] = f.y;
+        }
+      }
+      if (wp) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ss = fmaf(y[i], y[i], ss);
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float rs = rsqrtf(fmaf(ss, inv_d, a.eps));
+#pragma unroll
+        for (int i = 0; i < 16; ++i) y[i] *= rs * w[i];
+      }
+      if (rotates) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float& u = y[kInter ? 2 * i : i];
+          float& v = y[kInter ? 2 * i + 1 : 8 + i];
+          const float ua = u, va = v;
+          u = fmaf(ua, cs[i], -(va * sn[i]));
+          v = fmaf(va, cs[i], ua * sn[i]);
+        }
+      }
+      if (active && h < heads) {
+        uint16_t* r = out + t * o_row + h * o_head;
+        *reinterpret_cast<uint4*>(r + c0) =
+            make_uint4(dev::from_f2<kBf16>(y[0], y[1]), dev::from_f2<kBf16>(y[2], y[3]),
+                       dev::from_f2<kBf16>(y[4], y[5]), dev::from_f2<kBf16>(y[6], y[7]));
+        *reinterpret_cast<uint4*>(r + c1) =
+            make_uint4(dev::from_f2<kBf16>(y[8], y[9]), dev::from_f2<kBf16>(y[10], y[11]),
+                       dev::from_f2<kBf16>(y[12], y[13]), dev::from_f2<kBf16>(y[14], y[15]));
+      }
+    }
+  }
+}
+
+template <bool kBf16, int kLanes>
+int launch(const KittyQkNormRopeArgs& a, uint32_t* err, cudaStream_t s) {
+  constexpr int kHeads = 32 / kLanes * kPasses;
+  RopeShape sh;
+  sh.q_chunks = (a.num_q_heads + kHeads - 1) / kHeads;
+  sh.chunks = sh.q_chunks + (a.num_k_heads + kHeads - 1) / kHeads;
+  const int64_t warps = int64_t(a.rows) * sh.chunks, per = kThreads / 32;
+  // at least one warp for each chunk of heads, at most what the card holds at once
+  const int64_t most = std::max<int64_t>(int64_t(sm_count()) * 4, (sh.chunks + per - 1) / per);
+  const int64_t grid = std::min((warps + per - 1) / per, most);
+  if (a.interleaved) qk_norm_rope_kernel<kBf16, kLanes, true><<<unsigned(grid), kThreads, 0, s>>>(a, sh, err);
+  else qk_norm_rope_kernel<kBf16, kLanes, false><<<unsigned(grid), kThreads, 0, s>>>(a, sh, err);
+  return check_launch("qk_norm_rope");
+}
+
+template <bool kBf16>
+int launch_dim(const KittyQkNormRopeArgs& a, uint32_t* err, cudaStream_t s) {
+  if (a.head_dim <= 64) return launch<kBf16, 4>(a, err, s);
+  if (a.head_dim <= 128) return launch<kBf16, 8>(a, err, s);
+  return launch<kBf16, 16>(a, err, s);
+}
+
+}  // namespace
+}  // namespace kitty8
+
+using namespace kitty8;
+
+extern "C" int kitty_qk_norm_rope(const KittyQkNormRopeArgs* a, void* stream) {
+  const char* what = "qk_norm_rope";
+  if (!a) return fail(KITTY_ERR_INVALID_ARGUMENT, what, "args is NULL");
+  if (a->rows < 0 || a->num_q_heads < 0 || a->num_k_heads < 0 || a->head_dim <= 0 || a->rot < 0 || a->table_rows < 0)
+    return fail(KITTY_ERR_INVALID_ARGUMENT, what, "negative or zero size");
+  if (a->head_dim % 16 || a->head_dim > 256)
+    return fail(KITTY_ERR_UNSUPPORTED, what, "head_dim must be a multiple of 16 and at most 256");
+  if (a->rot % 16 || a->rot > a->head_dim)
+    return fail(KITTY_ERR_UNSUPPORTED, what, "the rotary width must be a multiple of 16 and at most head_dim");
+  if (a->dtype != KITTY_KV8_F16 && a->dtype != KITTY_KV8_BF16)
+    return fail(KITTY_ERR_INVALID_ARGUMENT, what, "dtype must be KITTY_KV8_F16 or KITTY_KV8_BF16");
+  if ((a->q_weight == nullptr) != (a->k_weight == nullptr))
+    return fail(KITTY_ERR_INVALID_ARGUMENT, what, "q_weight and k_weight go together");
+  if (a->rows == 0 || a->num_q_heads + a->num_k_heads == 0) return KITTY_OK;
+  if (!a->positions || (a->rot > 0 && !a->table)) return fail(KITTY_ERR_INVALID_ARGUMENT, what, "NULL positions or table");
+  if ((a->num_q_heads > 0 && (!a->q || !a->q_out)) || (a->num_k_heads > 0 && (!a->k || !a->k_out)))
+    return fail(KITTY_ERR_INVALID_ARGUMENT, what, "NULL q, k or outputs");
+  const int64_t strides[] = {a->q_s_row, a->q_s_head, a->k_s_row, a->k_s_head,
+                             a->qo_s_row, a->qo_s_head, a->ko_s_row, a->ko_s_head};
+  for (int64_t v : strides)
+    if (v % 8) return fail(KITTY_ERR_INVALID_ARGUMENT, what, "row and head strides must be multiples of 8 elements");
+  if (!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->q_out, 16) || !aligned(a->k_out, 16) ||
+      !aligned(a->table, 16))
+    return fail(KITTY_ERR_INVALID_ARGUMENT, what, "tensors must be 16-byte aligned");
+  uint32_t* err = error_word();
+  if (!err) return fail(KITTY_ERR_CUDA, what, "no CUDA device");
+  return a->dtype == KITTY_KV8_BF16 ? launch_dim<true>(*a, err, as_stream(stream))
+                                    : launch_dim<false>(*a, err, as_stream(stream));
+}
