@@ -6,7 +6,8 @@ Compiles every ``csrc/*.cu`` for sm_100a only (no PTX for other targets) with
 IEEE float32 division and square root (no --use_fast_math: the quantisers must
 round exactly like the reference) and links one shared library exporting the
 C ABI declared in ``include/kitty_b200.h``; ``csrc/kv8/*.cu`` (the 8-bit cache) make
-a second one with the C ABI of ``include/kitty_kv8.h``.  Objects go to ``_build/``.
+a second one with the C ABI of ``include/kitty_kv8.h``, and ``csrc/kv8/kv8_torch.cpp`` the
+Python module that calls it with torch tensors.  Objects go to ``_build/``.
 """
 
 from __future__ import annotations
@@ -15,6 +16,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -24,6 +26,7 @@ CSRC = PKG_ROOT / "csrc"
 BUILD = PKG_ROOT / "_build"
 LIB = PKG_ROOT / "kitty" / "libkitty_b200.so"
 LIB_KV8 = PKG_ROOT / "kitty" / "libkitty_kv8.so"
+KV8_TORCH = PKG_ROOT / "kitty" / "kernels" / "_kv8_torch.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -42,6 +45,7 @@ def build(verbose: bool = False, extra: list | None = None) -> Path:
     _library(LIB, CSRC.glob("*.cu"), headers, [], verbose, extra)
     headers = [*(CSRC / "kv8").glob("*.cuh"), *(REPO_ROOT / "include").glob("*.h")]
     _library(LIB_KV8, (CSRC / "kv8").glob("*.cu"), headers, ["-Xcompiler", "-fvisibility=hidden"], verbose, extra)
+    _torch_module(KV8_TORCH, CSRC / "kv8" / "kv8_torch.cpp", LIB_KV8, verbose)
     return LIB
 
 
@@ -63,11 +67,32 @@ def _library(lib: Path, sources, headers, flags: list, verbose: bool, extra: lis
             done.result()
     if (not lib.exists()) or any(o.stat().st_mtime > lib.stat().st_mtime for o in objs):
         tmp = lib.with_suffix(".so.tmp")
-        cmd = [nvcc(), *ARCH, "-shared", "-cudart", "static", "-o", str(tmp), *map(str, objs)]
+        cmd = [nvcc(), *ARCH, "-shared", "-cudart", "static", "-Xlinker", f"-soname={lib.name}", "-o", str(tmp),
+               *map(str, objs)]
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
         os.replace(tmp, lib)
+
+def _torch_module(module: Path, src: Path, lib: Path, verbose: bool) -> None:
+    """The Python extension module: the host compiler, torch's headers and libraries."""
+    header = REPO_ROOT / "include" / "kitty_kv8.h"
+    if module.exists() and module.stat().st_mtime >= max(src.stat().st_mtime, header.stat().st_mtime):
+        return
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parent.parent
+    tmp = module.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-isystem{d}" for d in (root / "include", root / "include" / "torch" / "csrc" / "api" / "include",
+                                      cuda / "include", sysconfig.get_paths()["include"])),
+           str(src), "-o", str(tmp), str(lib), "-Wl,-rpath,$ORIGIN/..", f"-L{root / 'lib'}",
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, module)
 
 
 if __name__ == "__main__":

@@ -1,8 +1,10 @@
 """ctypes binding of ``libkitty_kv8.so`` (the C ABI in ``include/kitty_kv8.h``).
 
 Loaded on first use, like ``libkitty_b200.so``: a missing library or one of another
-ABI version raises ``RuntimeError``, there is no fallback.  Entry points run on the
-current torch stream of the tensors' device, whichever device is the current one.
+ABI version raises ``RuntimeError``, there is no fallback.  The operators themselves go
+through :func:`ops`, which checks the tensors in C++ and runs the entry points on the
+current torch stream of the tensors' device, whichever device is the current one; the
+structs here are for callers that bind the C ABI themselves.
 """
 
 from __future__ import annotations
@@ -22,8 +24,6 @@ LIB_NAME = "libkitty_kv8.so"
 _LIB_PATH = Path(os.environ.get("KITTY_KV8_LIB", Path(__file__).resolve().parent.parent / LIB_NAME))
 
 ERROR_NAMES = {1: "invalid argument", 2: "unsupported", 3: "CUDA error", 4: "workspace"}
-DTYPES = {torch.float16: 0, torch.bfloat16: 1}
-CODES = {torch.float8_e4m3fn: 0, torch.int8: 1}
 
 # Sticky device error bits (kitty_kv8_error_flags).
 ERRORS = {1 << 1: "page number outside the pool or the block table", 1 << 2: "row offsets out of order or range",
@@ -118,15 +118,21 @@ def check(rc: int, what: str) -> None:
         raise RuntimeError(f"{what} failed ({ERROR_NAMES.get(rc, rc)}): {msg}")
 
 
-def launch(device: torch.device, name: str, args: ctypes.Structure) -> None:
-    """Run an entry point on the device's current torch stream."""
-    fn = getattr(load(), name)
-    if torch.cuda.current_device() == device.index:
-        rc = fn(args, torch.cuda.current_stream(device).cuda_stream)
-    else:
-        with torch.cuda.device(device):
-            rc = fn(args, torch.cuda.current_stream(device).cuda_stream)
-    check(rc, name)
+_ops = None
+
+
+def ops():
+    """The module that calls the entry points with torch tensors (``csrc/kv8/kv8_torch.cpp``)."""
+    global _ops
+    if _ops is None:
+        load()
+        try:
+            from . import _kv8_torch
+        except ImportError as e:
+            raise RuntimeError("Kitty's torch module for the 8-bit cache cannot be loaded. Build it with "
+                               f"`python kitty-kv_b200/build.py` (there is no CPU fallback): {e}") from e
+        _ops = _kv8_torch
+    return _ops
 
 
 def error_flags(device: torch.device, clear: bool = True) -> int:

@@ -23,57 +23,11 @@ CUDA graph.  No backward passes.
 
 from __future__ import annotations
 
-import math
 from typing import Optional, Tuple
 
 import torch
 
-from . import _kv8, _lib
-from .rope import aligned_rows, no_grad_inputs, output_rows
-
-
-def _fill_cache(c: _kv8.Cache, lengths, block_table, key_codes, value_codes, key_scale, value_scale, tail_k,
-                tail_v) -> None:
-    """Check the arrays of a cache against one another and describe them to the library."""
-    if key_codes.dim() != 4 or value_codes.shape != key_codes.shape:
-        raise RuntimeError("key_codes and value_codes must both be (P, H, G, D)")
-    pages, h, g, d = key_codes.shape
-    code = _kv8.CODES.get(key_codes.dtype)
-    if code is None or value_codes.dtype != key_codes.dtype:
-        raise RuntimeError("key_codes and value_codes must both be float8_e4m3fn or both int8")
-    slots = lengths.shape[0] if lengths.dim() == 1 else -1
-    if lengths.dtype != torch.int32 or slots < 0:
-        raise RuntimeError("lengths must be (slots,) int32")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != slots:
-        raise RuntimeError("block_table must be (slots, M) int32 with a row for each entry of lengths")
-    if block_table.shape[1] > 1 and block_table.stride(1) != 1:
-        raise RuntimeError("block_table rows need unit stride")
-    dt = _kv8.DTYPES.get(tail_k.dtype)
-    if dt is None or tail_v.dtype != tail_k.dtype:
-        raise RuntimeError("tail_k and tail_v must both be float16 or both bfloat16")
-    if tail_k.shape != (slots, h, g, d) or tail_v.shape != tail_k.shape:
-        raise RuntimeError(f"tail_k and tail_v must be ({slots}, {h}, {g}, {d})")
-    if key_scale.dtype != torch.float32 or value_scale.dtype != torch.float32 or key_scale.shape != (pages, h) or \
-            value_scale.shape != (pages, h):
-        raise RuntimeError(f"key_scale and value_scale must be ({pages}, {h}) float32")
-    if not (key_codes.is_contiguous() and value_codes.is_contiguous() and key_scale.is_contiguous() and
-            value_scale.is_contiguous() and tail_k.is_contiguous() and tail_v.is_contiguous() and
-            lengths.is_contiguous()):
-        raise RuntimeError("pools, scales, tails and lengths must be contiguous")
-    c.key_codes, c.value_codes = key_codes.data_ptr(), value_codes.data_ptr()
-    c.key_scale, c.value_scale = key_scale.data_ptr(), value_scale.data_ptr()
-    c.tail_k, c.tail_v = tail_k.data_ptr(), tail_v.data_ptr()
-    c.block_table, c.lengths = block_table.data_ptr(), lengths.data_ptr()
-    c.bt_s_slot, c.pages, c.slots, c.max_pages = block_table.stride(0), pages, slots, block_table.shape[1]
-    c.num_heads, c.head_dim, c.page_size, c.code, c.dtype = h, d, g, code, dt
-
-
-def _index(t: Optional[torch.Tensor], name: str, n: int) -> Optional[torch.Tensor]:
-    if t is None:
-        return None
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n:
-        raise RuntimeError(f"{name} must be ({n},) int32")
-    return t.contiguous()
+from . import _kv8
 
 
 def write_kv8(key: torch.Tensor, value: torch.Tensor, lengths: torch.Tensor, block_table: torch.Tensor,
@@ -89,26 +43,8 @@ def write_kv8(key: torch.Tensor, value: torch.Tensor, lengths: torch.Tensor, blo
     is not changed: add the new tokens before the next call on this cache.  Rows behind
     the last offset are ignored.
     """
-    dev = _lib.require_cuda(key, value, lengths, block_table, key_codes, value_codes, key_scale, value_scale, tail_k,
-                            tail_v, row_offsets, seq_map)
-    no_grad_inputs(key, value)
-    a = _kv8.WriteArgs()
-    _fill_cache(a.cache, lengths, block_table, key_codes, value_codes, key_scale, value_scale, tail_k, tail_v)
-    if key.dim() != 3 or key.shape != value.shape or tuple(key.shape[1:]) != (a.cache.num_heads, a.cache.head_dim) or \
-            key.dtype != tail_k.dtype or value.dtype != tail_k.dtype:
-        raise RuntimeError(f"key and value must be (N, {a.cache.num_heads}, {a.cache.head_dim}) {tail_k.dtype}")
-    rows = key.shape[0]
-    n = seq_map.numel() if seq_map is not None else rows if row_offsets is None else row_offsets.numel() - 1
-    if n < 0:
-        raise RuntimeError("row_offsets must have n + 1 entries")
-    if row_offsets is None and n != rows:
-        raise RuntimeError("without row_offsets key and value must have one row for each slot")
-    seq_map, row_offsets = _index(seq_map, "seq_map", n), _index(row_offsets, "row_offsets", n + 1)
-    key, a.k_s_row, a.k_s_head = aligned_rows(key)
-    value, a.v_s_row, a.v_s_head = aligned_rows(value)
-    a.key, a.value, a.n, a.rows = key.data_ptr(), value.data_ptr(), n, rows
-    a.row_offsets, a.seq_map = _lib.ptr(row_offsets), _lib.ptr(seq_map)
-    _kv8.launch(dev, "kitty_kv8_write", a)
+    _kv8.ops().write(key, value, lengths, block_table, key_codes, value_codes, key_scale, value_scale, tail_k, tail_v,
+                     row_offsets, seq_map)
 
 
 def read_kv8(lengths: torch.Tensor, block_table: torch.Tensor, key_codes: torch.Tensor, value_codes: torch.Tensor,
@@ -123,27 +59,8 @@ def read_kv8(lengths: torch.Tensor, block_table: torch.Tensor, key_codes: torch.
     last offset, and rows of tokens that the slot does not have, are left as they were
     (``key_out`` / ``value_out``: the caller's tensors, contiguous).
     """
-    dev = _lib.require_cuda(lengths, block_table, key_codes, value_codes, key_scale, value_scale, tail_k, tail_v,
-                            row_offsets, first, seq_map, key_out, value_out)
-    a = _kv8.ReadArgs()
-    _fill_cache(a.cache, lengths, block_table, key_codes, value_codes, key_scale, value_scale, tail_k, tail_v)
-    n = row_offsets.numel() - 1
-    if n < 0 or rows < 0:
-        raise RuntimeError("row_offsets must have n + 1 entries and rows must not be negative")
-    row_offsets, first, seq_map = _index(row_offsets, "row_offsets", n + 1), _index(first, "first", n), _index(
-        seq_map, "seq_map", n)
-    shape = (rows, a.cache.num_heads, a.cache.head_dim)
-    if key_out is None:
-        key_out = torch.empty(shape, dtype=tail_k.dtype, device=dev)
-    if value_out is None:
-        value_out = torch.empty(shape, dtype=tail_k.dtype, device=dev)
-    for t, name in ((key_out, "key_out"), (value_out, "value_out")):
-        if t.shape != shape or t.dtype != tail_k.dtype or not t.is_contiguous():
-            raise RuntimeError(f"{name} must be {shape} {tail_k.dtype}, contiguous")
-    a.key, a.value, a.n, a.rows = key_out.data_ptr(), value_out.data_ptr(), n, rows
-    a.row_offsets, a.first, a.seq_map = row_offsets.data_ptr(), _lib.ptr(first), _lib.ptr(seq_map)
-    _kv8.launch(dev, "kitty_kv8_read", a)
-    return key_out, value_out
+    return _kv8.ops().read(lengths, block_table, key_codes, value_codes, key_scale, value_scale, tail_k, tail_v,
+                           row_offsets, rows, first, seq_map, key_out, value_out)
 
 
 def paged_attention_kv8(q: torch.Tensor, lengths: torch.Tensor, block_table: torch.Tensor, key_codes: torch.Tensor,
@@ -158,30 +75,8 @@ def paged_attention_kv8(q: torch.Tensor, lengths: torch.Tensor, block_table: tor
     zeros.  Two launches; the scratch they share is allocated for each call, so calls on
     several streams or in several graphs do not meet.
     """
-    dev = _lib.require_cuda(q, lengths, block_table, key_codes, value_codes, key_scale, value_scale, tail_k, tail_v,
-                            seq_map, out)
-    no_grad_inputs(q)
-    a = _kv8.AttentionArgs()
-    _fill_cache(a.cache, lengths, block_table, key_codes, value_codes, key_scale, value_scale, tail_k, tail_v)
-    h, d = a.cache.num_heads, a.cache.head_dim
-    if q.dim() != 3 or q.shape[2] != d or q.dtype != tail_k.dtype:
-        raise RuntimeError(f"q must be (B, Hq, {d}) {tail_k.dtype}")
-    b, hq, _ = q.shape
-    if hq == 0 or hq % h:
-        raise RuntimeError("num_q_heads must be a multiple of num_kv_heads")
-    seq_map = _index(seq_map, "seq_map", b)
-    if out is None:
-        out = torch.empty((b, hq, d), dtype=q.dtype, device=dev)
-    a.out_s_seq, a.out_s_head = output_rows(out, q, "out")
-    q, a.q_s_seq, a.q_s_head = aligned_rows(q)
-    a.q, a.out, a.seq_map, a.batch, a.num_q_heads = q.data_ptr(), out.data_ptr(), _lib.ptr(seq_map), b, hq
-    a.sm_scale = 1.0 / math.sqrt(d) if sm_scale is None else float(sm_scale)
-    nbytes = _lib.c_size(0)
-    _kv8.check(_kv8.load().kitty_kv8_attention_workspace_size(a, nbytes), "kitty_kv8_attention_workspace_size")
-    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes.value
-    _kv8.launch(dev, "kitty_kv8_attention", a)
-    return out
+    return _kv8.ops().attention(q, lengths, block_table, key_codes, value_codes, key_scale, value_scale, tail_k, tail_v,
+                                sm_scale, seq_map, out)
 
 
 def kv8_error_flags(device: Optional[torch.device] = None, clear: bool = True) -> int:

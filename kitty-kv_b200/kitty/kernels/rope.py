@@ -11,7 +11,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from . import _kv8, _lib
+from . import _kv8
 
 
 def rope_table(max_positions: int, rotary_dim: int, base: float = 10000.0,
@@ -33,39 +33,6 @@ def rope_table(max_positions: int, rotary_dim: int, base: float = 10000.0,
     return torch.cat([angle.cos(), angle.sin()], dim=1).to(torch.float32)
 
 
-def aligned_rows(t: torch.Tensor) -> Tuple[torch.Tensor, int, int]:
-    """t ((rows, heads, D)) with 16-byte aligned rows, copied if it has none, and its row
-    and head strides in elements."""
-    n, h, d = t.shape
-    s0, s1, s2 = t.stride()
-    s0, s1 = (s0 if n > 1 else 0), (s1 if h > 1 else 0)
-    if s2 != 1 or s0 % 8 or s1 % 8 or t.data_ptr() % 16:
-        t = t.clone(memory_format=torch.contiguous_format)
-        s0, s1 = h * d, d
-    return t, s0, s1
-
-
-def output_rows(t: torch.Tensor, like: torch.Tensor, name: str) -> Tuple[int, int]:
-    """Row and head strides of a caller's output tensor; refused if its rows are not
-    aligned or overlap."""
-    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
-        raise RuntimeError(f"{name} must be {tuple(like.shape)} {like.dtype} on {like.device}")
-    n, h, _ = t.shape
-    s0, s1, s2 = t.stride()
-    if (n > 1 and s0 == 0) or (h > 1 and s1 == 0):
-        raise RuntimeError(f"{name} has rows that overlap")
-    s0, s1 = (s0 if n > 1 else 0), (s1 if h > 1 else 0)
-    if s2 != 1 or s0 % 8 or s1 % 8 or t.data_ptr() % 16:
-        raise RuntimeError(f"{name} needs unit channel stride and 16-byte aligned rows")
-    return s0, s1
-
-
-def no_grad_inputs(*tensors: Optional[torch.Tensor]) -> None:
-    """These operators have no backward pass: refuse inputs that ask for one."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("this operator has no backward pass: call it under torch.no_grad() or on detached tensors")
-
-
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: torch.Tensor,
                  q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
                  eps: float = 1e-6, interleaved: bool = False, q_out: Optional[torch.Tensor] = None,
@@ -83,43 +50,4 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
     q_out / k_out: given tensors, also q and k themselves (same strides); q and k may be
     strided views, as of one fused projection.  D and R are multiples of 16, D <= 256.
     """
-    dev = _lib.require_cuda(q, k, positions, table, q_weight, k_weight, q_out, k_out)
-    no_grad_inputs(q, k, q_weight, k_weight, table)
-    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
-        raise RuntimeError("q must be (N, Hq, D) and k (N, H, D)")
-    dt = _kv8.DTYPES.get(q.dtype)
-    if dt is None or k.dtype != q.dtype:
-        raise RuntimeError(f"q and k must both be float16 or both bfloat16, got {q.dtype} and {k.dtype}")
-    n, hq, d = q.shape
-    if positions.dtype not in (torch.int32, torch.int64) or positions.shape != (n,):
-        raise RuntimeError(f"positions must be ({n},) int32 or int64")
-    if table.dim() != 2 or table.dtype != torch.float32 or not table.is_contiguous():
-        raise RuntimeError("table must be (max_positions, R) float32, contiguous")
-    if (q_weight is None) != (k_weight is None):
-        raise RuntimeError("q_weight and k_weight must be given together")
-    w32 = False
-    if q_weight is not None:
-        if q_weight.shape != (d,) or k_weight.shape != (d,):
-            raise RuntimeError(f"q_weight and k_weight must be ({d},)")
-        w32 = q_weight.dtype == torch.float32
-        if k_weight.dtype != q_weight.dtype or not (w32 or q_weight.dtype == q.dtype):
-            raise RuntimeError(f"q_weight and k_weight must both be {q.dtype} or both float32")
-        q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
-    positions = positions.contiguous()
-    a = _kv8.QkNormRopeArgs()
-    if q_out is None:
-        q_out = torch.empty((n, hq, d), dtype=q.dtype, device=dev)
-    if k_out is None:
-        k_out = torch.empty((n, k.shape[1], d), dtype=q.dtype, device=dev)
-    a.qo_s_row, a.qo_s_head = output_rows(q_out, q, "q_out")
-    a.ko_s_row, a.ko_s_head = output_rows(k_out, k, "k_out")
-    q, a.q_s_row, a.q_s_head = aligned_rows(q)
-    k, a.k_s_row, a.k_s_head = aligned_rows(k)
-    a.q, a.k, a.q_out, a.k_out = q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr()
-    a.q_weight, a.k_weight = _lib.ptr(q_weight), _lib.ptr(k_weight)
-    a.positions, a.table, a.table_rows = positions.data_ptr(), table.data_ptr(), table.shape[0]
-    a.rows, a.num_q_heads, a.num_k_heads, a.head_dim, a.rot = n, hq, k.shape[1], d, table.shape[1]
-    a.interleaved, a.positions64, a.weight_f32 = interleaved, positions.dtype == torch.int64, w32
-    a.dtype, a.eps = dt, eps
-    _kv8.launch(dev, "kitty_qk_norm_rope", a)
-    return q_out, k_out
+    return _kv8.ops().qk_norm_rope(q, k, positions, table, q_weight, k_weight, eps, interleaved, q_out, k_out)
