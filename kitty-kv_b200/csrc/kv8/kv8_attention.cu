@@ -25,11 +25,14 @@
 // headroom; for fp16 outputs, whose own rounding is as small, they are split in two
 // parts (16-bit tails of bf16 slots: two bf16 parts).
 //
-// All segments' tiles (kTile tokens of a page, 16 of a tail) are laid end to end and every
-// warp of a fixed grid takes one contiguous slice; warps never wait for one another.  The
+// All segments' tiles (kTile tokens of a page, half as many of a tail: about the same
+// bytes) are laid end to end, each segment's behind kSetup units that stand for what a
+// segment costs a warp besides its tiles, and every warp of a fixed grid takes one
+// contiguous slice of the units; warps never wait for one another over the data.  The
 // next tile's keys are requested when this tile's scores are done, its values when this
-// tile's output is.  A segment inside one slice is stored at once; the parts of one that
-// crosses slices go to the workspace (two places a warp) and are joined by merge_kernel.
+// tile's output is.  A segment inside one slice is stored at once; of one that crosses
+// slices every warp leaves a part in the workspace (two places a warp), or, where all
+// warps of a CTA work on it, the CTA leaves one, and merge_kernel joins them.
 #include "kv8_common.cuh"
 
 namespace kitty8 {
@@ -38,6 +41,8 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kHead = 14.f;          // weights are kept times 2^kHead, so that small ones stay normal in fp16
 constexpr int kWarps = 4;              // per CTA
+constexpr int kSetup = 2;              // units (tiles) that beginning and ending a segment count as
+constexpr int kAhead = 4;              // tiles that a prefetch asks for
 constexpr int kMergeThreads = 256;
 
 struct Plan {
@@ -103,116 +108,263 @@ __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t
 // Tiles of a slot's segments: its whole pages, then its tail.
 struct Tiles {
   int paged, all, tail;                // tiles in pages, all tiles, tail tokens
+  __device__ int units() const { return all ? all + kSetup : 0; }
 };
 template <int kTile>
 __device__ __forceinline__ Tiles tiles_of(const KittyKv8Cache& c, int len) {
-  const int blocks = min(len / c.page_size, c.max_pages), tail = len % c.page_size;
+  const int blocks = len / c.page_size, tail = len - blocks * c.page_size;
   const int paged = blocks * (c.page_size / kTile);
-  return Tiles{paged, paged + (tail + 15) / 16, tail};
-}
-__device__ __forceinline__ int slot_of(const KittyKv8AttentionArgs& a, int b, uint32_t* err) {
-  const int s = a.seq_map ? a.seq_map[b] : b;
-  if (s >= 0 && s < a.cache.slots) return s;
-  if (err) dev::flag(err, kErrSlot);
-  return -1;
+  return Tiles{paged, paged + (tail + kTile / 2 - 1) / (kTile / 2), tail};
 }
 // Tokens of batch row b: 0 where its slot or its length is out of range.
 __device__ __forceinline__ int tokens_of(const KittyKv8AttentionArgs& a, int b, uint32_t* err = nullptr) {
-  const int s = slot_of(a, b, err);
-  if (s < 0) return 0;
+  const int s = a.seq_map ? a.seq_map[b] : b;
+  if (s < 0 || s >= a.cache.slots) {
+    if (err) dev::flag(err, kErrSlot);
+    return 0;
+  }
   const int len = a.cache.lengths[s];
   if (len >= 0 && len / a.cache.page_size <= a.cache.max_pages) return len;
   if (err) dev::flag(err, kErrLength);
   return 0;
 }
 
-struct Place {
-  int64_t total;       // tiles of the whole batch
-  int64_t begin;       // first tile of the segment found
-  int b, seg;          // its batch row; its index among the row's segments; b < 0: none
-};
+// a / b for non-negative a and positive b, in 32 bits where they fit (the 64-bit quotient is
+// a long sequence on the way to a warp's first load).
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? int64_t(uint32_t(a) / uint32_t(b)) : a / b;
+}
 
-// By the whole warp: all tiles, and the segment that holds tile f.  Row b has
-// `per_row` = H * passes segments of equal length.
+// The units of the whole batch, and where batch row `b` or unit `f` lies among them.  Row
+// b has `per_row` = H * passes segments of equal length.  By the whole warp.
+struct Place {
+  int64_t total;       // units of all rows
+  int64_t begin;       // first unit of the segment found
+  int b, seg;          // its batch row and its index among the row's segments
+};
 template <int kTile>
-__device__ __forceinline__ Place locate(const KittyKv8AttentionArgs& a, int per_row, int64_t f) {
+__device__ __forceinline__ int units_of_row(const KittyKv8AttentionArgs& a, int b, uint32_t* err = nullptr) {
+  return b < a.batch ? tiles_of<kTile>(a.cache, tokens_of(a, b, err)).units() : 0;
+}
+template <int kTile>
+__device__ __forceinline__ int64_t total_units(const KittyKv8AttentionArgs& a, int first, int per_row) {
   const int lane = threadIdx.x & 31;
-  Place r{0, 0, -1, 0};
+  int64_t sum = first;
+#pragma unroll 4
+  for (int b = lane + 32; b < a.batch; b += 32) sum += units_of_row<kTile>(a, b);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum * per_row;
+}
+// The segment that holds unit f (f < total); `first`: the units of row `lane`.
+template <int kTile>
+__device__ __forceinline__ Place locate(const KittyKv8AttentionArgs& a, int first, int per_row, int64_t f) {
+  const int lane = threadIdx.x & 31;
+  Place r{0, 0, 0, 0};
+  int64_t before = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 32) {
-    const int b = b0 + lane;
-    const int one = b < a.batch ? tiles_of<kTile>(a.cache, tokens_of(a, b)).all : 0;
-    const int64_t mine = int64_t(one) * per_row;
-    int64_t incl = mine;
+    const int one = b0 == 0 ? first : units_of_row<kTile>(a, b0 + lane);
+    int64_t incl = int64_t(one) * per_row;
+    const int64_t mine = incl;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += v;
     }
-    const int64_t start = r.total + incl - mine;
+    const int64_t start = before + incl - mine;
     const uint32_t hit = __ballot_sync(0xffffffffu, f >= start && f < start + mine);
     if (hit) {
       const int src = __ffs(hit) - 1;
       const int64_t at = __shfl_sync(0xffffffffu, start, src);
       const int len = __shfl_sync(0xffffffffu, one, src);
       r.b = b0 + src;
-      r.seg = int((f - at) / len);
+      r.seg = int(quotient(f - at, len));
       r.begin = at + int64_t(r.seg) * len;
+      return r;
     }
-    r.total += __shfl_sync(0xffffffffu, incl, 31);
+    before += __shfl_sync(0xffffffffu, incl, 31);
   }
   return r;
 }
 
+// Whether all warps of the CTA that holds warp w work on the segment [begin, end) only.
+__device__ __forceinline__ bool cta_inside(int64_t cta, int64_t per_warp, int64_t begin, int64_t end) {
+  return cta * kWarps * per_warp >= begin + kSetup && (cta + 1) * kWarps * per_warp <= end;
+}
+
+// Warps hide one another's latency, so the registers are capped for 12 warps an SM at 128
+// channels (8 without a cap: 345 against 330 us for 32 x 32K tokens) and 16 at 64 (88 us for
+// the mixed batch at 12, 80 at 16, 81 at 20).
+template <int kDim>
+constexpr int kMinCtas = kDim == 64 ? 4 : kDim == 128 ? 3 : 1;
+
 // kDim: 64, 128 or 256 channels in registers; kWhole: head_dim == kDim (else the missing
 // channels read as zero).  kNT: tiles of 8 query heads.
 template <int kDim, int kNT, bool kWhole, bool kBf16, int kCode>
-__global__ void __launch_bounds__(kWarps * 32) attention_kernel(KittyKv8AttentionArgs a, Plan plan, uint32_t* err) {
+__global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
+    attention_kernel(KittyKv8AttentionArgs a, Plan plan, uint32_t* err) {
   constexpr int kTile = kDim == 256 ? 16 : 32;      // tokens of a page tile
-  constexpr int kMT = kTile / 16;                   // 16-token groups of it
+  constexpr int kTailTile = kTile / 2;              // tokens of a tail tile
+  constexpr int kMT = kTile / 16;                   // 16-token groups of a page tile
   constexpr int kKC = kDim / 64;                    // 64-channel column blocks of a key row
   constexpr int kVH = kDim == 256 ? 2 : 1;          // 128-channel halves of a value row
   constexpr int kVW = kDim == 64 ? 2 : 4;           // words of codes a lane loads of a value row's half
   constexpr int kOT = kDim / 16;                    // output tiles
   constexpr int kParts = kBf16 ? 1 : 2;             // fp16 parts of a weight in the paged tiles
+  constexpr int kTailRows = kTailTile / 8;          // token rows of a score tile that a tail tile fills
+  __shared__ float4 s_o[kNT * kOT][kWarps][32];     // outputs of the CTA's warps where they share a segment
+  __shared__ float s_m[kWarps][kNT * 8], s_l[kWarps][kNT * 8];
   const KittyKv8Cache& c = a.cache;
   const int lane = threadIdx.x & 31, lr = lane >> 2, lc = lane & 3;
   const int warp = blockIdx.x * kWarps + (threadIdx.x >> 5);
   const int D = kWhole ? kDim : c.head_dim, G = c.page_size, H = c.num_heads;
   const int g = a.num_q_heads / H;
-  const int per_row = H * plan.passes;
+  const int per_row = H * plan.passes, per_block = G / kTile;
+  asm volatile("griddepcontrol.launch_dependents;");   // merge_kernel may start to look where its parts will be
+  const float fac16 = a.sm_scale * kLog2e;
 
   // this warp's slice [f, f_end)
+  const int first = units_of_row<kTile>(a, lane, warp == 0 ? err : nullptr);
   if (warp == 0)
-    for (int b = lane; b < a.batch; b += 32) tokens_of(a, b, err);
-  Place at = locate<kTile>(a, per_row, -1);
-  const int64_t per_warp = (at.total + plan.warps - 1) / plan.warps;
-  int64_t f = warp * per_warp;
-  const int64_t f_end = min(at.total, f + per_warp);
-  if (f >= f_end) return;
-  at = locate<kTile>(a, per_row, f);
+    for (int b = lane + 32; b < a.batch; b += 32) tokens_of(a, b, err);
+  const int64_t total = total_units<kTile>(a, first, per_row);
+  const int64_t per_warp = quotient(total + plan.warps - 1, plan.warps);
+  const int64_t f0 = warp * per_warp, f_end = min(total, f0 + per_warp);
+  if (f0 >= f_end) return;
+  const Place at = locate<kTile>(a, first, per_row, f0);
   int b = at.b, seg = at.seg;
   int64_t begin = at.begin;
 
-  while (f < f_end) {
+  while (begin < f_end) {
     const int len = tokens_of(a, b);
     const Tiles tl = tiles_of<kTile>(c, len);
-    if (tl.all == 0) { ++b; seg = 0; continue; }    // (f < total: a later row has tiles)
+    if (tl.all == 0) { ++b; continue; }             // (units are left, so a later row has some)
     const int slot = a.seq_map ? a.seq_map[b] : b;
-    const int h = seg / plan.passes, q0 = (seg % plan.passes) * plan.pass_heads;
+    const int h = seg / plan.passes, q0 = (seg - h * plan.passes) * plan.pass_heads;
     const int heads = min(plan.pass_heads, g - q0);
-    const int64_t seg_end = begin + tl.all;
-    const int t0 = int(f - begin), t1 = int(min(f_end, seg_end) - begin);   // this warp's tiles of the segment
-    const int p1 = min(t1, tl.paged);               // its tiles in pages end here
+    const int64_t end = begin + tl.units(), here = begin;
+    // this warp's tiles of the segment
+    const int t0 = int(max(f0 - here - kSetup, int64_t(0))), t1 = int(min(f_end, end) - here) - kSetup;
+    const int row_b = b;
+    begin = end;
+    if (++seg == per_row) { seg = 0; ++b; }
+    if (t0 >= t1) continue;                         // only setup units
 
-    // q: lane (lr, lc) holds head lr's channels 64 jj + 16 lc + 0..15 of each column block
+    // ---- the tiles' loads
+    uint4 kr[kMT * 2 * kKC];                        // keys: codes [group][row lr, lr + 8][column block], tail rows
+    uint32_t vr[kMT * kVH * 4 * kVW];               // values: codes [group][half][token][word], tail rows
+    float ks = 0.f, vs = 0.f;
+    bool ok = true;
+    int page = 0, sub = t0 % per_block, block = t0 / per_block;
+    const int last_block = (min(t1, tl.paged) - 1) / per_block;     // (not used without paged tiles)
+    const int32_t* table = c.block_table + int64_t(slot) * c.bt_s_slot;
+    int win0 = block;                               // the lanes hold 32 block-table entries from win0 on
+    int win = t0 < tl.paged && win0 + lane <= last_block ? table[win0 + lane] : 0;
+    const int64_t tail_base = (int64_t(slot) * H + h) * G * D;
+    // page of `block`: page 0 and not ok if it is no page of the pool
+    auto turn_page = [&]() {
+      if (block >= win0 + 32) {
+        win0 = block;
+        win = win0 + lane <= last_block ? table[win0 + lane] : 0;
+      }
+      page = __shfl_sync(0xffffffffu, win, block - win0);
+      ok = page >= 0 && page < c.pages;
+      if (!ok) {
+        if (lane == 0) dev::flag(err, kErrPage);
+        page = 0;
+      }
+    };
+    // Ask L2 for the page's next tiles, where it has at least kAhead of them: the loads of a
+    // tile find the following ones on their way.  Two tiles a page gain nothing by it (330
+    // against 330 us for 32 x 32K tokens at G = 64), four do (737 -> 686 us for 16 x 131K at
+    // G = 128); asking for more than 16 KB a warp costs (344 us at G = 64 for 32 KB).
+    auto prefetch = [&]() {
+      if (per_block >= kAhead && sub % kAhead == 0 && lane < 2) {
+        const int64_t at = ((int64_t(page) * H + h) * G + sub * kTile) * D;
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;"
+                     :: "l"(static_cast<const uint8_t*>(lane ? c.value_codes : c.key_codes) + at),
+                        "r"(min(kAhead, per_block - sub) * kTile * D));
+      }
+    };
+    auto load_keys = [&]() {
+      const uint8_t* p = static_cast<const uint8_t*>(c.key_codes) +
+                         ((int64_t(page) * H + h) * G + sub * kTile + lr) * D + 16 * lc;
+#pragma unroll
+      for (int r = 0; r < kMT * 2; ++r)
+#pragma unroll
+        for (int jj = 0; jj < kKC; ++jj)
+          kr[r * kKC + jj] = kWhole || 64 * jj + 16 * lc < D ? ld_stream(p + r * 8 * D + 64 * jj)
+                                                             : make_uint4(0, 0, 0, 0);
+      ks = __ldg(c.key_scale + int64_t(page) * H + h);
+    };
+    auto load_tail_keys = [&](int t) {
+      const int tok = (t - tl.paged) * kTailTile + lr;
+      const uint16_t* p = static_cast<const uint16_t*>(c.tail_k) + tail_base + tok * D + 16 * lc;
+#pragma unroll
+      for (int r = 0; r < kTailRows; ++r)
+#pragma unroll
+        for (int jj = 0; jj < kKC; ++jj) {
+          const bool there = tok + 8 * r < tl.tail && (kWhole || 64 * jj + 16 * lc < D);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            kr[(r * kKC + jj) * 2 + i] = there ? ld_stream(p + r * 8 * D + 64 * jj + 8 * i) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    auto load_values = [&]() {
+      const uint8_t* p = static_cast<const uint8_t*>(c.value_codes) +
+                         ((int64_t(page) * H + h) * G + sub * kTile + 2 * lc) * D + 4 * kVW * lr;
+#pragma unroll
+      for (int mt = 0; mt < kMT; ++mt)
+#pragma unroll
+        for (int vh = 0; vh < kVH; ++vh)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint8_t* x = p + (mt * 16 + (k / 2) * 8 + k % 2) * D + 128 * vh;
+            const bool there = kWhole || 128 * vh + 4 * kVW * lr < D;
+            uint32_t* v = vr + ((mt * kVH + vh) * 4 + k) * kVW;
+            if constexpr (kVW == 4) {
+              const uint4 u = there ? ld_stream(x) : make_uint4(0, 0, 0, 0);
+              v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+            } else {
+              const uint2 u = there ? ld_stream2(x) : make_uint2(0, 0);
+              v[0] = u.x; v[1] = u.y;
+            }
+          }
+      vs = __ldg(c.value_scale + int64_t(page) * H + h);
+    };
+    auto load_tail_values = [&](int t) {
+      // rows behind the tail's end may hold anything: they read as zero
+#pragma unroll
+      for (int vh = 0; vh < kVH; ++vh)
+#pragma unroll
+        for (int k = 0; k < 2 * kTailRows; ++k) {
+          const int row = (t - tl.paged) * kTailTile + 2 * lc + (k / 2) * 8 + k % 2;
+          const bool there = row < tl.tail && (kWhole || 128 * vh + 4 * kVW * lr < D);
+          const uint16_t* x = static_cast<const uint16_t*>(c.tail_v) + tail_base + row * D + 128 * vh + 4 * kVW * lr;
+#pragma unroll
+          for (int i = 0; i < kVW / 2; ++i) {
+            const uint4 u = there ? ld_stream(x + 8 * i) : make_uint4(0, 0, 0, 0);
+            uint32_t* v = vr + ((vh * 2 * kTailRows + k) * (kVW / 2) + i) * 4;
+            v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+          }
+        }
+    };
+    const int p1 = min(t1, tl.paged);               // tiles in pages end here
+    if (t0 < p1) {
+      turn_page();
+      prefetch();
+      load_keys();
+      load_values();
+    } else {
+      load_tail_keys(t0);
+      load_tail_values(t0);
+    }
+
+    // ---- q: lane (lr, lc) holds head lr's channels 64 jj + 16 lc + 0..15 of each column block
     const uint16_t* qrow[kNT];
     uint32_t qf[kNT][4 * kKC][2];
     float fac[kNT][2];                              // of the two columns (heads) whose scores this lane gets
-#pragma unroll
-    for (int nt = 0; nt < kNT; ++nt) {
-      const int qh = nt * 8 + lr;
-      qrow[nt] = qh < heads ? static_cast<const uint16_t*>(a.q) + b * a.q_s_seq + (h * g + q0 + qh) * a.q_s_head : nullptr;
-      float top = 0.f;
+    auto load_q = [&](int nt) {
 #pragma unroll
       for (int jj = 0; jj < kKC; ++jj) {
         uint4 u = make_uint4(0, 0, 0, 0), v = u;
@@ -223,35 +375,40 @@ __global__ void __launch_bounds__(kWarps * 32) attention_kernel(KittyKv8Attentio
         }
         const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          qf[nt][4 * jj + i / 2][i % 2] = w[i];
-          if constexpr (kBf16) {
-            const float2 x = dev::to_f2<true>(w[i]);
-            top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
-          }
-        }
+        for (int i = 0; i < 8; ++i) qf[nt][4 * jj + i / 2][i % 2] = w[i];
       }
+    };
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) {
+      const int qh = nt * 8 + lr;
+      qrow[nt] = qh < heads ? static_cast<const uint16_t*>(a.q) + row_b * a.q_s_seq + (h * g + q0 + qh) * a.q_s_head
+                            : nullptr;
+      load_q(nt);
       float scale = 1.f;                            // of head lr
       if constexpr (kBf16) {
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // 2^(14 - exponent): the largest element lands in [2^14, 2^15); an all-zero or
-        // infinite row keeps its values
-        const int e = int(__float_as_uint(top) >> 23);
-        const float up = e > 0 && e < 255 ? __uint_as_float(uint32_t(min(max(127 + 14 + 127 - e, 1), 254)) << 23) : 1.f;
-        scale = 1.f / up;                           // a power of two (or its subnormal neighbour's inverse): exact
+        if (t0 < tl.paged) {
+          float top = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4 * kKC; ++i) {
+          for (int i = 0; i < 8 * kKC; ++i) {
+            const float2 x = dev::to_f2<true>(qf[nt][i / 2][i % 2]);
+            top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
+          }
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          // 2^(14 - exponent): the largest element lands in [2^14, 2^15); an all-zero or
+          // infinite row keeps its values
+          const int e = int(__float_as_uint(top) >> 23);
+          const float up = e > 0 && e < 255 ? __uint_as_float(uint32_t(min(max(127 + 14 + 127 - e, 1), 254)) << 23) : 1.f;
+          scale = 1.f / up;                         // a power of two: exact
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float2 x = dev::to_f2<true>(qf[nt][i][k]);
-            qf[nt][i][k] = dev::from_f2<false>(x.x * up, x.y * up);
+          for (int i = 0; i < 8 * kKC; ++i) {
+            const float2 x = dev::to_f2<true>(qf[nt][i / 2][i % 2]);
+            qf[nt][i / 2][i % 2] = dev::from_f2<false>(x.x * up, x.y * up);
           }
         }
       }
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        fac[nt][j] = __shfl_sync(0xffffffffu, scale, (2 * lc + j) * 4) * (a.sm_scale * kLog2e);
+      for (int j = 0; j < 2; ++j) fac[nt][j] = __shfl_sync(0xffffffffu, scale, (2 * lc + j) * 4) * fac16;
     }
 
     float o[kNT][kOT][4], m[kNT][2], l[kNT][2];
@@ -264,8 +421,8 @@ __global__ void __launch_bounds__(kWarps * 32) attention_kernel(KittyKv8Attentio
     }
 
     // Softmax step of one tile: scores s (token rows lr and lr + 8 of each group, two head
-    // columns) become weights 2^(s - m + kHead), the sums are brought up to date and
-    // alpha gets the factor of what was there before.
+    // columns) become weights 2^(s - m + kHead) and alpha gets the factor of what was
+    // there before.
     auto softmax = [&](auto& s, int nt, float (&alpha)[2]) {
       constexpr int kGroups = sizeof(s) / sizeof(s[0]);
 #pragma unroll
@@ -287,277 +444,252 @@ __global__ void __launch_bounds__(kWarps * 32) attention_kernel(KittyKv8Attentio
       }
     };
 
-    // ------------------------------------------------------------------ pages
-    if (t0 < p1) {
-      const int per_block = G / kTile;
-      const int32_t* table = c.block_table + int64_t(slot) * c.bt_s_slot;
-      int win0 = t0 / per_block;                    // the lanes hold 32 block-table entries from win0 on
-      const int last_block = (p1 - 1) / per_block;
-      int win = win0 + lane <= last_block ? table[win0 + lane] : 0;
-      // block of a tile -> page (0 and not ok if it is no page of the pool)
-      auto page_at = [&](int block, bool& ok) {
-        if (block >= win0 + 32) {
-          win0 = block;
-          win = win0 + lane <= last_block ? table[win0 + lane] : 0;
-        }
-        const int p = __shfl_sync(0xffffffffu, win, block - win0);
-        ok = p >= 0 && p < c.pages;
-        if (!ok && lane == 0) dev::flag(err, kErrPage);
-        return ok ? p : 0;
-      };
-      uint4 kr[kMT][2][kKC];
-      uint32_t vr[kMT][kVH][4][kVW];
-      float ks, vs;
-      auto load_keys = [&](int page, int sub) {
-        const uint8_t* p = static_cast<const uint8_t*>(c.key_codes) +
-                           ((int64_t(page) * H + h) * G + sub * kTile + lr) * D + 16 * lc;
+    for (int t = t0; t < p1; ++t) {
+      // ------------------------------------------------------------ kTile tokens of a page
+      float s[kNT][kMT][4];
 #pragma unroll
-        for (int mt = 0; mt < kMT; ++mt)
+      for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-          for (int r = 0; r < 2; ++r)
+        for (int mt = 0; mt < kMT; ++mt) s[nt][mt][0] = s[nt][mt][1] = s[nt][mt][2] = s[nt][mt][3] = 0.f;
 #pragma unroll
-            for (int jj = 0; jj < kKC; ++jj)
-              kr[mt][r][jj] = kWhole || 64 * jj + 16 * lc < D ? ld_stream(p + (mt * 16 + r * 8) * D + 64 * jj)
-                                                              : make_uint4(0, 0, 0, 0);
-        ks = __ldg(c.key_scale + int64_t(page) * H + h);
-      };
-      auto load_values = [&](int page, int sub) {
-        const uint8_t* p = static_cast<const uint8_t*>(c.value_codes) +
-                           ((int64_t(page) * H + h) * G + sub * kTile + 2 * lc) * D + 4 * kVW * lr;
+      for (int jj = 0; jj < kKC; ++jj)
 #pragma unroll
-        for (int mt = 0; mt < kMT; ++mt)
+        for (int mt = 0; mt < kMT; ++mt) {
+          const uint4 u0 = kr[(2 * mt) * kKC + jj], u1 = kr[(2 * mt + 1) * kKC + jj];
+          const uint32_t w0[4] = {u0.x, u0.y, u0.z, u0.w}, w1[4] = {u1.x, u1.y, u1.z, u1.w};
 #pragma unroll
-          for (int vh = 0; vh < kVH; ++vh)
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              const uint8_t* at_ = p + (mt * 16 + (t / 2) * 8 + t % 2) * D + 128 * vh;
-              const bool there = kWhole || 128 * vh + 4 * kVW * lr < D;
-              if constexpr (kVW == 4) {
-                const uint4 u = there ? ld_stream(at_) : make_uint4(0, 0, 0, 0);
-                vr[mt][vh][t][0] = u.x; vr[mt][vh][t][1] = u.y; vr[mt][vh][t][2] = u.z; vr[mt][vh][t][3] = u.w;
-              } else {
-                const uint2 u = there ? ld_stream2(at_) : make_uint2(0, 0);
-                vr[mt][vh][t][0] = u.x; vr[mt][vh][t][1] = u.y;
-              }
-            }
-        vs = __ldg(c.value_scale + int64_t(page) * H + h);
-      };
-
-      bool ok;
-      int page = page_at(t0 / per_block, ok);
-      load_keys(page, t0 % per_block);
-      load_values(page, t0 % per_block);
-      for (int t = t0; t < p1; ++t) {
-        float s[kNT][kMT][4];
-#pragma unroll
-        for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-          for (int mt = 0; mt < kMT; ++mt) s[nt][mt][0] = s[nt][mt][1] = s[nt][mt][2] = s[nt][mt][3] = 0.f;
-#pragma unroll
-        for (int jj = 0; jj < kKC; ++jj)
-#pragma unroll
-          for (int mt = 0; mt < kMT; ++mt) {
-            const uint32_t w0[4] = {kr[mt][0][jj].x, kr[mt][0][jj].y, kr[mt][0][jj].z, kr[mt][0][jj].w};
-            const uint32_t w1[4] = {kr[mt][1][jj].x, kr[mt][1][jj].y, kr[mt][1][jj].z, kr[mt][1][jj].w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t a0, a1, a2, a3;
-              codes_to_half<kCode>(w0[i], a0, a2);
-              codes_to_half<kCode>(w1[i], a1, a3);
-#pragma unroll
-              for (int nt = 0; nt < kNT; ++nt)
-                mma<false>(s[nt][mt], a0, a1, a2, a3, qf[nt][4 * jj + i][0], qf[nt][4 * jj + i][1]);
-            }
-          }
-        const float ks_now = ks, vs_now = vs;
-        const bool ok_now = ok;
-        const bool more = t + 1 < p1;
-        const int sub = (t + 1) % per_block;
-        if (more) {
-          if (sub == 0) page = page_at((t + 1) / per_block, ok);
-          load_keys(page, sub);
-        }
-        uint32_t wb[kNT][kMT][kParts][2];           // weights as the other operand: tokens 0..7 and 8..15 of a group
-        float alpha[kNT][2];
-#pragma unroll
-        for (int nt = 0; nt < kNT; ++nt) {
-#pragma unroll
-          for (int mt = 0; mt < kMT; ++mt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[nt][mt][i] = ok_now ? s[nt][mt][i] * (fac[nt][i & 1] * ks_now) : -INFINITY;
-          softmax(s[nt], nt, alpha[nt]);
-          float sum[2] = {0.f, 0.f};
-#pragma unroll
-          for (int mt = 0; mt < kMT; ++mt)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const uint32_t hi = dev::from_f2<false>(s[nt][mt][2 * r], s[nt][mt][2 * r + 1]);
-              const float2 back = dev::to_f2<false>(hi);
-              wb[nt][mt][0][r] = transpose8x8(hi);
-              if constexpr (kParts == 2) {
-                wb[nt][mt][kParts - 1][r] =
-                    transpose8x8(dev::from_f2<false>(s[nt][mt][2 * r] - back.x, s[nt][mt][2 * r + 1] - back.y));
-                sum[0] += s[nt][mt][2 * r];
-                sum[1] += s[nt][mt][2 * r + 1];
-              } else {                              // the sum of what the product uses
-                sum[0] += back.x;
-                sum[1] += back.y;
-              }
-            }
-          l[nt][0] = l[nt][0] * alpha[nt][0] + sum[0];
-          l[nt][1] = l[nt][1] * alpha[nt][1] + sum[1];
-        }
-        const float vmul = ok_now ? vs_now : 0.f;
-#pragma unroll
-        for (int vh = 0; vh < kVH; ++vh)
-#pragma unroll
-          for (int x = 0; x < kVW; ++x)
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {           // bytes 0, 1 or 2, 3 of the word: two channels
-              const uint32_t sel = y ? 0x7362u : 0x5140u;
-              const int i = (vh * kVW + x) * 2 + y;
-              float acc[kNT][4];
-#pragma unroll
-              for (int nt = 0; nt < kNT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
-#pragma unroll
-              for (int mt = 0; mt < kMT; ++mt) {
-                uint32_t a0, a1, a2, a3;
-                codes_to_half<kCode>(prmt(vr[mt][vh][0][x], vr[mt][vh][1][x], sel), a0, a1);
-                codes_to_half<kCode>(prmt(vr[mt][vh][2][x], vr[mt][vh][3][x], sel), a2, a3);
-#pragma unroll
-                for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-                  for (int p = 0; p < kParts; ++p)
-                    mma<false>(acc[nt], a0, a1, a2, a3, wb[nt][mt][p][0], wb[nt][mt][p][1]);
-              }
-#pragma unroll
-              for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[nt][i][e] = fmaf(acc[nt][e], vmul, o[nt][i][e] * alpha[nt][e & 1]);
-            }
-        if (more) load_values(page, sub);
-      }
-    }
-
-    // ------------------------------------------------------------------ tail: 16 tokens of 16 bits a tile
-    if (t1 > tl.paged) {
-      if constexpr (kBf16) {                        // q as it is: bf16 products
-#pragma unroll
-        for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-          for (int jj = 0; jj < kKC; ++jj) {
-            uint4 u = make_uint4(0, 0, 0, 0), v = u;
-            const int ch = 64 * jj + 16 * lc;
-            if (qrow[nt] && (kWhole || ch < D)) {
-              u = *reinterpret_cast<const uint4*>(qrow[nt] + ch);
-              v = *reinterpret_cast<const uint4*>(qrow[nt] + ch + 8);
-            }
-            const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int i = 0; i < 8; ++i) qf[nt][4 * jj + i / 2][i % 2] = w[i];
-          }
-      }
-      const int64_t base = (int64_t(slot) * H + h) * G * D;
-      const uint16_t* tk = static_cast<const uint16_t*>(c.tail_k) + base;
-      const uint16_t* tv = static_cast<const uint16_t*>(c.tail_v) + base;
-      const float fac16 = a.sm_scale * kLog2e;
-      for (int t = max(t0, tl.paged); t < t1; ++t) {
-        const int tok = (t - tl.paged) * 16;
-        float s[kNT][1][4];
-#pragma unroll
-        for (int nt = 0; nt < kNT; ++nt) s[nt][0][0] = s[nt][0][1] = s[nt][0][2] = s[nt][0][3] = 0.f;
-        const bool row0 = tok + lr < tl.tail, row1 = tok + lr + 8 < tl.tail;
-#pragma unroll
-        for (int jj = 0; jj < kKC; ++jj) {
-          const uint4 z = make_uint4(0, 0, 0, 0);
-          uint4 u[2][2] = {{z, z}, {z, z}};
-          const int ch = 64 * jj + 16 * lc;
-          if (kWhole || ch < D) {
-            const uint16_t* p = tk + (tok + lr) * D + ch;
-            if (row0) { u[0][0] = ld_stream(p); u[0][1] = ld_stream(p + 8); }
-            if (row1) { u[1][0] = ld_stream(p + 8 * D); u[1][1] = ld_stream(p + 8 * D + 8); }
-          }
-          const uint32_t w0[8] = {u[0][0].x, u[0][0].y, u[0][0].z, u[0][0].w, u[0][1].x, u[0][1].y, u[0][1].z, u[0][1].w};
-          const uint32_t w1[8] = {u[1][0].x, u[1][0].y, u[1][0].z, u[1][0].w, u[1][1].x, u[1][1].y, u[1][1].z, u[1][1].w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < 4; ++i) {
+            uint32_t a0, a1, a2, a3;
+            codes_to_half<kCode>(w0[i], a0, a2);
+            codes_to_half<kCode>(w1[i], a1, a3);
 #pragma unroll
             for (int nt = 0; nt < kNT; ++nt)
-              mma<kBf16>(s[nt][0], w0[2 * i], w1[2 * i], w0[2 * i + 1], w1[2 * i + 1], qf[nt][4 * jj + i][0],
-                         qf[nt][4 * jj + i][1]);
+              mma<false>(s[nt][mt], a0, a1, a2, a3, qf[nt][4 * jj + i][0], qf[nt][4 * jj + i][1]);
+          }
         }
-        uint32_t wb[kNT][2][2];                     // two parts of the tails' type
-        float alpha[kNT][2];
+      const float ks_now = ks, vs_now = vs;
+      const bool ok_now = ok;
+      if (t + 1 < p1) {
+        if (++sub == per_block) {
+          sub = 0;
+          ++block;
+          turn_page();
+        }
+        prefetch();
+        load_keys();
+      } else if (t + 1 < t1) {
+        load_tail_keys(t + 1);
+      }
+      uint32_t wb[kNT][kMT][kParts][2];           // weights as the other operand: tokens 0..7 and 8..15 of a group
+      float alpha[kNT][2];
 #pragma unroll
-        for (int nt = 0; nt < kNT; ++nt) {
+      for (int nt = 0; nt < kNT; ++nt) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[nt][0][i] = (i < 2 ? row0 : row1) ? s[nt][0][i] * fac16 : -INFINITY;
-          softmax(s[nt], nt, alpha[nt]);
+        for (int mt = 0; mt < kMT; ++mt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[nt][mt][i] = ok_now ? s[nt][mt][i] * (fac[nt][i & 1] * ks_now) : -INFINITY;
+        softmax(s[nt], nt, alpha[nt]);
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const uint32_t hi = dev::from_f2<kBf16>(s[nt][0][2 * r], s[nt][0][2 * r + 1]);
-            const float2 back = dev::to_f2<kBf16>(hi);
-            wb[nt][0][r] = transpose8x8(hi);
-            wb[nt][1][r] = transpose8x8(dev::from_f2<kBf16>(s[nt][0][2 * r] - back.x, s[nt][0][2 * r + 1] - back.y));
-          }
-          l[nt][0] = l[nt][0] * alpha[nt][0] + (s[nt][0][0] + s[nt][0][2]);
-          l[nt][1] = l[nt][1] * alpha[nt][1] + (s[nt][0][1] + s[nt][0][3]);
-        }
-#pragma unroll
-        for (int vh = 0; vh < kVH; ++vh) {
-          // rows behind the tail's end may hold anything: they read as zero
-          uint32_t w[4][2 * kVW];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int row = tok + 2 * lc + (k / 2) * 8 + k % 2;
-            const bool there = row < tl.tail && (kWhole || 128 * vh + 4 * kVW * lr < D);
-            const uint16_t* p = tv + row * D + 128 * vh + 4 * kVW * lr;
-#pragma unroll
-            for (int q = 0; q < kVW / 2; ++q) {
-              const uint4 u = there ? ld_stream(p + 8 * q) : make_uint4(0, 0, 0, 0);
-              w[k][4 * q] = u.x; w[k][4 * q + 1] = u.y; w[k][4 * q + 2] = u.z; w[k][4 * q + 3] = u.w;
+            const uint32_t hi = dev::from_f2<false>(s[nt][mt][2 * r], s[nt][mt][2 * r + 1]);
+            const float2 back = dev::to_f2<false>(hi);
+            wb[nt][mt][0][r] = transpose8x8(hi);
+            if constexpr (kParts == 2) {
+              wb[nt][mt][kParts - 1][r] =
+                  transpose8x8(dev::from_f2<false>(s[nt][mt][2 * r] - back.x, s[nt][mt][2 * r + 1] - back.y));
+              sum[0] += s[nt][mt][2 * r];
+              sum[1] += s[nt][mt][2 * r + 1];
+            } else {                              // the sum of what the product uses
+              sum[0] += back.x;
+              sum[1] += back.y;
             }
           }
+        l[nt][0] = l[nt][0] * alpha[nt][0] + sum[0];
+        l[nt][1] = l[nt][1] * alpha[nt][1] + sum[1];
+      }
+      const float vmul = ok_now ? vs_now : 0.f;
 #pragma unroll
-          for (int x = 0; x < 2 * kVW; ++x) {       // a word holds the channel pair of one output tile
-            const int i = vh * kVW * 2 + x;
-            const uint32_t a0 = prmt(w[0][x], w[1][x], 0x5410), a1 = prmt(w[0][x], w[1][x], 0x7632);
-            const uint32_t a2 = prmt(w[2][x], w[3][x], 0x5410), a3 = prmt(w[2][x], w[3][x], 0x7632);
+      for (int vh = 0; vh < kVH; ++vh)
 #pragma unroll
-            for (int nt = 0; nt < kNT; ++nt) {
+        for (int x = 0; x < kVW; ++x)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) o[nt][i][e] *= alpha[nt][e & 1];
-              mma<kBf16>(o[nt][i], a0, a1, a2, a3, wb[nt][0][0], wb[nt][0][1]);
-              mma<kBf16>(o[nt][i], a0, a1, a2, a3, wb[nt][1][0], wb[nt][1][1]);
+          for (int y = 0; y < 2; ++y) {           // bytes 0, 1 or 2, 3 of the word: two channels
+            const uint32_t sel = y ? 0x7362u : 0x5140u;
+            const int i = (vh * kVW + x) * 2 + y;
+            float acc[kNT][4];
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
+#pragma unroll
+            for (int mt = 0; mt < kMT; ++mt) {
+              const uint32_t* v = vr + (mt * kVH + vh) * 4 * kVW + x;
+              uint32_t a0, a1, a2, a3;
+              codes_to_half<kCode>(prmt(v[0], v[kVW], sel), a0, a1);
+              codes_to_half<kCode>(prmt(v[2 * kVW], v[3 * kVW], sel), a2, a3);
+#pragma unroll
+              for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+                for (int p = 0; p < kParts; ++p)
+                  mma<false>(acc[nt], a0, a1, a2, a3, wb[nt][mt][p][0], wb[nt][mt][p][1]);
             }
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[nt][i][e] = fmaf(acc[nt][e], vmul, o[nt][i][e] * alpha[nt][e & 1]);
           }
-        }
+      if (t + 1 < p1) load_values();
+      else if (t + 1 < t1) load_tail_values(t + 1);
+    }
+    if constexpr (kBf16) {                          // bf16 products in the tail: q as it is
+      if (t0 < p1 && p1 < t1) {
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) load_q(nt);
       }
     }
+    for (int t = max(t0, p1); t < t1; ++t) {
+      // ------------------------------------------------------------ kTailTile tokens of 16 bits
+      const int tok = (t - tl.paged) * kTailTile + lr;
+      float s[kNT][1][4];
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) s[nt][0][0] = s[nt][0][1] = s[nt][0][2] = s[nt][0][3] = 0.f;
+#pragma unroll
+      for (int jj = 0; jj < kKC; ++jj)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint4 u0 = kr[jj * 2 + i];
+          const uint4 u1 = kTailRows == 2 ? kr[((kTailRows - 1) * kKC + jj) * 2 + i] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int nt = 0; nt < kNT; ++nt) {
+            mma<kBf16>(s[nt][0], u0.x, u1.x, u0.y, u1.y, qf[nt][4 * jj + 2 * i][0], qf[nt][4 * jj + 2 * i][1]);
+            mma<kBf16>(s[nt][0], u0.z, u1.z, u0.w, u1.w, qf[nt][4 * jj + 2 * i + 1][0], qf[nt][4 * jj + 2 * i + 1][1]);
+          }
+        }
+      if (t + 1 < t1) load_tail_keys(t + 1);
+      uint32_t wb[kNT][2][2];                     // two parts of the tails' type
+      float alpha[kNT][2];
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          s[nt][0][i] = i / 2 < kTailRows && tok + 8 * (i / 2) < tl.tail ? s[nt][0][i] * fac16 : -INFINITY;
+        softmax(s[nt], nt, alpha[nt]);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint32_t hi = dev::from_f2<kBf16>(s[nt][0][2 * r], s[nt][0][2 * r + 1]);
+          const float2 back = dev::to_f2<kBf16>(hi);
+          wb[nt][0][r] = transpose8x8(hi);
+          wb[nt][1][r] = transpose8x8(dev::from_f2<kBf16>(s[nt][0][2 * r] - back.x, s[nt][0][2 * r + 1] - back.y));
+        }
+        l[nt][0] = l[nt][0] * alpha[nt][0] + (s[nt][0][0] + s[nt][0][2]);
+        l[nt][1] = l[nt][1] * alpha[nt][1] + (s[nt][0][1] + s[nt][0][3]);
+      }
+#pragma unroll
+      for (int vh = 0; vh < kVH; ++vh)
+#pragma unroll
+        for (int x = 0; x < 2 * kVW; ++x) {       // a word holds the channel pair of one output tile
+          const int i = vh * kVW * 2 + x;
+          const uint32_t* v = vr + vh * 2 * kTailRows * 2 * kVW + x;
+          const uint32_t a0 = prmt(v[0], v[2 * kVW], 0x5410), a1 = prmt(v[0], v[2 * kVW], 0x7632);
+          const uint32_t w2 = kTailRows == 2 ? v[(kTailRows - 1) * 4 * kVW] : 0u;
+          const uint32_t w3 = kTailRows == 2 ? v[(kTailRows - 1) * 6 * kVW] : 0u;
+          const uint32_t a2 = prmt(w2, w3, 0x5410), a3 = prmt(w2, w3, 0x7632);
+#pragma unroll
+          for (int nt = 0; nt < kNT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[nt][i][e] *= alpha[nt][e & 1];
+            mma<kBf16>(o[nt][i], a0, a1, a2, a3, wb[nt][0][0], wb[nt][0][1]);
+            mma<kBf16>(o[nt][i], a0, a1, a2, a3, wb[nt][1][0], wb[nt][1][1]);
+          }
+        }
+      if (t + 1 < t1) load_tail_values(t + 1);
+    }
 
-    // ------------------------------------------------------------------ store
-    const bool all_here = t0 == 0 && t1 == tl.all;
-    const int64_t place = 2 * int64_t(warp) + (f > warp * per_warp);   // the slice's first segment, or its last
+    // ---- store: the segment's output, or this warp's or CTA's part of it
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float sum = l[nt][j];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 4);
+        l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 8);
+        l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 16);
+      }
+    const bool all_here = t0 == 0 && t1 == tl.all;
+    const bool together = cta_inside(blockIdx.x, per_warp, here, end);
+    int x0 = 0, x1 = kOT / 2;                       // pairs of output tiles that this warp stores
+    const int w = threadIdx.x >> 5;
+    if (together) {
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) {
+#pragma unroll
+        for (int i = 0; i < kOT; ++i)
+          s_o[nt * kOT + i][w][lane] = make_float4(o[nt][i][0], o[nt][i][1], o[nt][i][2], o[nt][i][3]);
+        if (lr == 0) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            s_m[w][nt * 8 + 2 * lc + j] = m[nt][j];
+            s_l[w][nt * 8 + 2 * lc + j] = l[nt][j];
+          }
+        }
+      }
+      __syncthreads();                              // (each CTA comes here at most once: its slices lie in the segment)
+      constexpr int kEach = (kOT / 2 + kWarps - 1) / kWarps;
+      x0 = w * kEach;
+      x1 = min(x0 + kEach, kOT / 2);
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) {
+        float k[kWarps][2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int col = nt * 8 + 2 * lc + j;
+          float top = s_m[0][col];
+#pragma unroll
+          for (int i = 1; i < kWarps; ++i) top = fmaxf(top, s_m[i][col]);
+          const float ref = top == -INFINITY ? 0.f : top;
+          m[nt][j] = top;
+          l[nt][j] = 0.f;
+#pragma unroll
+          for (int i = 0; i < kWarps; ++i) {
+            k[i][j] = ex2(s_m[i][col] - ref);
+            l[nt][j] = fmaf(k[i][j], s_l[i][col], l[nt][j]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kOT; ++i) {
+          if (i / 2 < x0 || i / 2 >= x1) continue;
+          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int q = 0; q < kWarps; ++q) {
+            const float4 v = s_o[nt * kOT + i][q][lane];
+            sum.x = fmaf(k[q][0], v.x, sum.x);
+            sum.y = fmaf(k[q][1], v.y, sum.y);
+            sum.z = fmaf(k[q][0], v.z, sum.z);
+            sum.w = fmaf(k[q][1], v.w, sum.w);
+          }
+          o[nt][i][0] = sum.x; o[nt][i][1] = sum.y; o[nt][i][2] = sum.z; o[nt][i][3] = sum.w;
+        }
+      }
+    }
+    // the slice's first segment, or its last; of a CTA's warps together, the first's place
+    const int64_t place = together ? 2 * int64_t(blockIdx.x) * kWarps : 2 * int64_t(warp) + (here > f0);
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
         const int qh = nt * 8 + 2 * lc + j;
         if (qh >= heads) continue;
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        uint16_t* out = static_cast<uint16_t*>(a.out) + b * a.out_s_seq + (h * g + q0 + qh) * a.out_s_head;
+        const float inv = l[nt][j] == 0.f ? 0.f : 1.f / l[nt][j];
+        uint16_t* out = static_cast<uint16_t*>(a.out) + row_b * a.out_s_seq + (h * g + q0 + qh) * a.out_s_head;
         float* part = plan.part_o + (place * plan.pass_heads + qh) * D;
-        if (!all_here && lr == 0) {
+        if (!all_here && lr == 0 && x0 == 0) {
           float* ml = plan.part_ml + (place * plan.pass_heads + qh) * 2;
           ml[0] = m[nt][j];
-          ml[1] = sum;
+          ml[1] = l[nt][j];
         }
 #pragma unroll
         for (int x = 0; x < kOT / 2; ++x) {         // four channels from two output tiles
+          if (x < x0 || x >= x1) continue;
           const int vh = x / kVW, ch = 128 * vh + 4 * kVW * lr + 4 * (x % kVW);
           if (!kWhole && ch >= D) continue;
           const float v0 = o[nt][2 * x][j], v1 = o[nt][2 * x][2 + j], v2 = o[nt][2 * x + 1][j], v3 = o[nt][2 * x + 1][2 + j];
@@ -568,73 +700,80 @@ __global__ void __launch_bounds__(kWarps * 32) attention_kernel(KittyKv8Attentio
             *reinterpret_cast<float4*>(part + ch) = make_float4(v0, v1, v2, v3);
         }
       }
-    f = begin + t1;
-    if (f == seg_end) {
-      begin = seg_end;
-      if (++seg == per_row) { seg = 0; ++b; }
-    }
   }
 }
 
-// One CTA per segment: joins the parts that its warps left, out = sum_i 2^(m_i - M) O_i /
-// sum_i 2^(m_i - M) l_i; zeros for an empty slot.  The threads form groups of D / 4 (one
-// 16-byte vector of a part each); the groups share the parts and are summed in order.
-template <int kTile, bool kBf16>
+// Joins the parts of a segment: out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i; zeros
+// for an empty slot.  Where segments are few, each has many parts: a CTA takes one query
+// head of one (kTeam threads), its threads form groups of one thread for each 16-byte
+// vector of the head, the groups take the parts in turn, each with its own maximum, and
+// are joined in order.  Where they are many, most have one part and nothing to join: a warp
+// takes all heads of one.
+template <int kTile, bool kBf16, int kTeam>
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(KittyKv8AttentionArgs a, Plan plan) {
-  extern __shared__ float4 s_sum[];                 // [groups][heads * D / 4]
-  __shared__ float s_l[kMergeThreads];
+  __shared__ float4 s_sum[kTeam == 32 ? 1 : kTeam];
+  __shared__ float s_l[kTeam == 32 ? 1 : kTeam], s_m[kTeam == 32 ? 1 : kTeam];
   const KittyKv8Cache& c = a.cache;
+  const int lane = threadIdx.x & 31, tid = threadIdx.x % kTeam;
   const int D = c.head_dim, g = a.num_q_heads / c.num_heads, per_row = c.num_heads * plan.passes;
-  const int b = blockIdx.x / per_row, seg = blockIdx.x % per_row;
-  const int h = seg / plan.passes, q0 = (seg % plan.passes) * plan.pass_heads;
-  const int heads = min(plan.pass_heads, g - q0);
-  // where the segment lies among all tiles
+  const int64_t segment = int64_t(blockIdx.x) * (kMergeThreads / kTeam) + threadIdx.x / kTeam;
+  const int b = int(segment / per_row), seg = int(segment - int64_t(b) * per_row);
+  const int h = seg / plan.passes, q0 = (seg - h * plan.passes) * plan.pass_heads;
+  const int first_head = kTeam == 32 ? 0 : blockIdx.y;
+  const int heads = kTeam == 32 ? min(plan.pass_heads, g - q0) : (first_head < g - q0 ? 1 : 0);
+  // where the segment lies among all units
   int64_t before = 0, total = 0;
-  {
-    const int lane = threadIdx.x & 31;
-    for (int i = lane; i < a.batch; i += 32) {
-      const int64_t n = tiles_of<kTile>(c, tokens_of(a, i)).all;
-      total += n;
-      if (i < b) before += n;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      total += __shfl_xor_sync(0xffffffffu, total, o);
-      before += __shfl_xor_sync(0xffffffffu, before, o);
-    }
-    total *= per_row;
-    before *= per_row;
+#pragma unroll 4
+  for (int i = lane; i < a.batch; i += 32) {
+    const int64_t n = units_of_row<kTile>(a, i);
+    total += n;
+    if (i < b) before += n;
   }
-  const int tiles = tiles_of<kTile>(c, tokens_of(a, b)).all;
-  uint16_t* out = static_cast<uint16_t*>(a.out) + b * a.out_s_seq + int64_t(h * g + q0) * a.out_s_head;
-  const int vecs = D / 4;
-  if (tiles == 0) {
-    for (int u = threadIdx.x; u < heads * vecs; u += kMergeThreads)
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+  }
+  total *= per_row;
+  before *= per_row;
+  const int units = units_of_row<kTile>(a, b);
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // attention_kernel is done and its parts are visible
+  if (b >= a.batch || heads <= 0) return;
+  uint16_t* out = static_cast<uint16_t*>(a.out) + b * a.out_s_seq + int64_t(h * g + q0 + first_head) * a.out_s_head;
+  const int vecs = D / 4, work = heads * vecs;
+  if (units == 0) {
+    for (int u = tid; u < work; u += kTeam)
       *reinterpret_cast<uint2*>(out + (u / vecs) * a.out_s_head + (u % vecs) * 4) = make_uint2(0, 0);
     return;
   }
-  const int64_t per_warp = (total + plan.warps - 1) / plan.warps;
-  const int64_t begin = before + int64_t(seg) * tiles, end = begin + tiles;
-  const int w0 = int(begin / per_warp), w1 = int((end - 1) / per_warp);
+  const int64_t per_warp = quotient(total + plan.warps - 1, plan.warps), per_cta = per_warp * kWarps;
+  const int64_t begin = before + int64_t(seg) * units, end = begin + units;
+  const int w0 = int(quotient(begin + kSetup, per_warp)), w1 = int(quotient(end - 1, per_warp));
   if (w0 == w1) return;                             // stored by its warp
-  const bool inside = begin > w0 * per_warp;        // it is the last of w0's slice, not the first
-  auto place = [&](int w) { return 2 * int64_t(w) + (w == w0 && inside); };
-  const int units = heads * vecs;
-  const int groups = max(1, kMergeThreads / units);
-  for (int u0 = 0; u0 < units; u0 += kMergeThreads) {
-    const int group = units <= kMergeThreads ? threadIdx.x / units : 0;
-    const int u = u0 + (units <= kMergeThreads ? threadIdx.x % units : threadIdx.x);
-    const bool work = u < units && group < groups;
-    const int qh = work ? u / vecs : 0, v = u % vecs;
-    float top = -INFINITY;
-    for (int w = w0; w <= w1; ++w) top = fmaxf(top, plan.part_ml[(place(w) * plan.pass_heads + qh) * 2]);
-    const float ref = top == -INFINITY ? 0.f : top;
+  // its parts: warps w0 .., whole CTAs c0 .. c1 - 1, warps .. w1
+  const int c0 = int(quotient(begin + kSetup + per_cta - 1, per_cta)), c1 = int(quotient(end, per_cta));
+  const int n2 = max(c1 - c0, 0);
+  const int n1 = n2 ? c0 * kWarps - w0 : w1 - w0 + 1;
+  const int parts = n2 ? n1 + n2 + (w1 - c1 * kWarps + 1) : n1;
+  auto place = [&](int i) {
+    const int w = i < n1 ? w0 + i : i < n1 + n2 ? (c0 + i - n1) * kWarps : c1 * kWarps + (i - n1 - n2);
+    return (2 * int64_t(w) + (begin > w * per_warp)) * plan.pass_heads + first_head;
+  };
+  const int groups = kTeam == 32 ? 1 : kTeam / vecs;  // (vecs <= 64)
+  for (int u0 = 0; u0 < work; u0 += kTeam) {        // (a CTA's team has one round: work == vecs)
+    const int group = kTeam == 32 ? 0 : tid / vecs;
+    const int u = kTeam == 32 ? u0 + tid : tid - group * vecs;
+    const bool mine = u < work && group < groups;
+    const int qh = mine ? u / vecs : 0, v = mine ? u - qh * vecs : 0;
+    float top = -INFINITY, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
-    if (work) {
+    if (mine) {
 #pragma unroll 4
-      for (int w = w0 + group; w <= w1; w += groups) {
-        const int64_t at = place(w) * plan.pass_heads + qh;
+      for (int i = group; i < parts; i += groups) top = fmaxf(top, plan.part_ml[(place(i) + qh) * 2]);
+      const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll 4
+      for (int i = group; i < parts; i += groups) {
+        const int64_t at = place(i) + qh;
         const float k = ex2(plan.part_ml[at * 2] - ref);
         const float4 p = *reinterpret_cast<const float4*>(plan.part_o + at * D + v * 4);
         sum = fmaf(k, plan.part_ml[at * 2 + 1], sum);
@@ -644,23 +783,49 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(KittyKv8AttentionA
         acc.w = fmaf(k, p.w, acc.w);
       }
     }
-    if (groups > 1) {
-      s_sum[threadIdx.x] = acc;
-      s_l[threadIdx.x] = sum;
+    if constexpr (kTeam != 32) {
+      s_sum[tid] = acc;
+      s_l[tid] = sum;
+      s_m[tid] = top;
       __syncthreads();
-      if (work && group == 0)
-        for (int k = 1; k < groups; ++k) {
-          const float4 p = s_sum[k * units + u];
-          acc.x += p.x; acc.y += p.y; acc.z += p.z; acc.w += p.w;
-          sum += s_l[k * units + u];
+      if (mine && group == 0) {
+        for (int k = 1; k < groups; ++k) top = fmaxf(top, s_m[k * vecs + u]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        sum = 0.f;
+        for (int k = 0; k < groups; ++k) {
+          const float f = ex2(s_m[k * vecs + u] - ref);
+          const float4 p = s_sum[k * vecs + u];
+          sum = fmaf(f, s_l[k * vecs + u], sum);
+          acc.x = fmaf(f, p.x, acc.x);
+          acc.y = fmaf(f, p.y, acc.y);
+          acc.z = fmaf(f, p.z, acc.z);
+          acc.w = fmaf(f, p.w, acc.w);
         }
+      }
     }
-    if (work && group == 0) {
+    if (mine && group == 0) {
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       *reinterpret_cast<uint2*>(out + qh * a.out_s_head + v * 4) =
           make_uint2(dev::from_f2<kBf16>(acc.x * inv, acc.y * inv), dev::from_f2<kBf16>(acc.z * inv, acc.w * inv));
     }
   }
+}
+
+// merge_kernel behind attention_kernel, as its programmatic dependent: it is launched while
+// the other runs and waits in front of the first part that it reads.
+template <int kTile, bool kBf16, int kTeam>
+cudaError_t launch_merge(const KittyKv8AttentionArgs& a, const Plan& plan, dim3 grid, cudaStream_t s) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = kMergeThreads;
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, merge_kernel<kTile, kBf16, kTeam>, a, plan);
 }
 
 // Resident CTAs per SM that a kernel's registers allow (asked once per kernel).
@@ -694,9 +859,14 @@ int launch(const KittyKv8AttentionArgs& a, Plan plan, uint32_t* err, cudaStream_
   const int rc = check_launch("kv8_attention");
   if (rc != KITTY_OK) return rc;
   constexpr int kTile = kDim == 256 ? 16 : 32;
+  // Few segments are shared by many warps each, many segments are mostly one warp's own.
   const unsigned segments = unsigned(a.batch) * a.cache.num_heads * plan.passes;
-  merge_kernel<kTile, kBf16><<<segments, kMergeThreads, kMergeThreads * sizeof(float4), s>>>(a, plan);
-  return check_launch("kv8_attention (merge)");
+  const unsigned per = kMergeThreads / 32;
+  const cudaError_t e =
+      segments < unsigned(plan.warps) / 4
+          ? launch_merge<kTile, kBf16, kMergeThreads>(a, plan, dim3(segments, unsigned(plan.pass_heads)), s)
+          : launch_merge<kTile, kBf16, 32>(a, plan, dim3((segments + per - 1) / per), s);
+  return e == cudaSuccess ? KITTY_OK : fail(KITTY_ERR_CUDA, "kv8_attention (merge)", cudaGetErrorString(e));
 }
 
 template <int kDim, bool kWhole, bool kBf16, int kCode>
