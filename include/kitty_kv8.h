@@ -138,7 +138,7 @@ typedef struct KittyKv8AttentionArgs {
 } KittyKv8AttentionArgs;
 
 /* Bytes of workspace that kitty_kv8_attention needs for these arguments (it depends on
- * the shapes alone, not on the lengths or the batch). */
+ * the shapes alone, not on the lengths). */
 int kitty_kv8_attention_workspace_size(const KittyKv8AttentionArgs* args, size_t* bytes);
 int kitty_kv8_attention(const KittyKv8AttentionArgs* args, void* stream);
 

@@ -44,12 +44,15 @@ constexpr int kWarps = 4;              // per CTA
 constexpr int kSetup = 2;              // units (tiles) that beginning and ending a segment count as
 constexpr int kAhead = 4;              // tiles that a prefetch asks for
 constexpr int kMergeThreads = 256;
+constexpr int kBatch = 8;              // parts whose loads merge_kernel has in flight
 
 struct Plan {
   int passes, pass_heads;              // query heads of a KV head in passes of pass_heads
   int warps;                           // of the whole grid
   float* part_ml;                      // [2 warps][pass_heads][2]  maximum, sum
   float* part_o;                       // [2 warps][pass_heads][D]
+  int64_t* seg_begin;                  // [segments] first unit of a segment that left parts, -1: stored; then the
+                                       // units of a slice
 };
 
 __device__ __forceinline__ uint4 ld_stream(const void* p) {
@@ -231,6 +234,7 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
   const int64_t per_warp = quotient(total + plan.warps - 1, plan.warps);
   const int64_t f0 = warp * per_warp, f_end = min(total, f0 + per_warp);
   if (f0 >= f_end) return;
+  if (warp == 0 && lane == 0) plan.seg_begin[int64_t(a.batch) * per_row] = per_warp;
   const Place at = locate<kTile>(a, first, per_row, f0);
   int b = at.b, seg = at.seg;
   int64_t begin = at.begin;
@@ -246,6 +250,7 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
     // this warp's tiles of the segment
     const int t0 = int(max(f0 - here - kSetup, int64_t(0))), t1 = int(min(f_end, end) - here) - kSetup;
     const int row_b = b;
+    const int64_t segment = int64_t(b) * per_row + seg;
     begin = end;
     if (++seg == per_row) { seg = 0; ++b; }
     if (t0 >= t1) continue;                         // only setup units
@@ -616,6 +621,7 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
         l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 16);
       }
     const bool all_here = t0 == 0 && t1 == tl.all;
+    if (t0 == 0 && lane == 0) plan.seg_begin[segment] = all_here ? -1 : here;
     const bool together = cta_inside(blockIdx.x, per_warp, here, end);
     int x0 = 0, x1 = kOT / 2;                       // pairs of output tiles that this warp stores
     const int w = threadIdx.x >> 5;
@@ -703,53 +709,59 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
   }
 }
 
-// Joins the parts of a segment: out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i; zeros
-// for an empty slot.  Where segments are few, each has many parts: a CTA takes one query
-// head of one (kTeam threads), its threads form groups of one thread for each 16-byte
-// vector of the head, the groups take the parts in turn, each with its own maximum, and
-// are joined in order.  Where they are many, most have one part and nothing to join: a warp
-// takes all heads of one.
+// Joins the parts of a segment's query head: out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M)
+// l_i; zeros for an empty slot.  Where segments are few, each has many parts: the team is
+// a CTA, whose threads form groups of one thread for each 16-byte vector of the head; the
+// groups take the parts in turn, each with its own maximum, and are joined in order.  Where
+// they are many, most were stored by their warp and the others have a few parts: the team is
+// a warp.
 template <int kTile, bool kBf16, int kTeam>
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(KittyKv8AttentionArgs a, Plan plan) {
   __shared__ float4 s_sum[kTeam == 32 ? 1 : kTeam];
   __shared__ float s_l[kTeam == 32 ? 1 : kTeam], s_m[kTeam == 32 ? 1 : kTeam];
   const KittyKv8Cache& c = a.cache;
-  const int lane = threadIdx.x & 31, tid = threadIdx.x % kTeam;
+  const int tid = threadIdx.x % kTeam;
   const int D = c.head_dim, g = a.num_q_heads / c.num_heads, per_row = c.num_heads * plan.passes;
-  const int64_t segment = int64_t(blockIdx.x) * (kMergeThreads / kTeam) + threadIdx.x / kTeam;
-  const int b = int(segment / per_row), seg = int(segment - int64_t(b) * per_row);
+  const uint32_t team = blockIdx.x * (kMergeThreads / kTeam) + threadIdx.x / kTeam;
+  const uint32_t segment = team / plan.pass_heads;
+  const int head = int(team - segment * plan.pass_heads);
+  const int b = int(segment / per_row), seg = int(segment - uint32_t(b) * per_row);
   const int h = seg / plan.passes, q0 = (seg - h * plan.passes) * plan.pass_heads;
-  const int first_head = kTeam == 32 ? 0 : blockIdx.y;
-  const int heads = kTeam == 32 ? min(plan.pass_heads, g - q0) : (first_head < g - q0 ? 1 : 0);
-  // where the segment lies among all units
-  int64_t before = 0, total = 0;
-#pragma unroll 4
-  for (int i = lane; i < a.batch; i += 32) {
-    const int64_t n = units_of_row<kTile>(a, i);
-    total += n;
-    if (i < b) before += n;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    total += __shfl_xor_sync(0xffffffffu, total, o);
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-  }
-  total *= per_row;
-  before *= per_row;
   const int units = units_of_row<kTile>(a, b);
+  // Where the segment begins: a few rows are looked through while attention_kernel still
+  // runs, of many the kernel has left a note.
+  int64_t begin = -1, per_warp = 1;
+  if constexpr (kTeam != 32) {
+    int64_t before = 0, total = 0;
+    for (int i = threadIdx.x & 31; i < a.batch; i += 32) {
+      const int64_t n = units_of_row<kTile>(a, i);
+      total += n;
+      if (i < b) before += n;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      total += __shfl_xor_sync(0xffffffffu, total, o);
+      before += __shfl_xor_sync(0xffffffffu, before, o);
+    }
+    per_warp = max(quotient(total * per_row + plan.warps - 1, plan.warps), int64_t(1));
+    begin = before * per_row + int64_t(seg) * units;
+  }
   asm volatile("griddepcontrol.wait;" ::: "memory");   // attention_kernel is done and its parts are visible
-  if (b >= a.batch || heads <= 0) return;
-  uint16_t* out = static_cast<uint16_t*>(a.out) + b * a.out_s_seq + int64_t(h * g + q0 + first_head) * a.out_s_head;
-  const int vecs = D / 4, work = heads * vecs;
+  if (b >= a.batch || q0 + head >= g) return;
+  uint16_t* out = static_cast<uint16_t*>(a.out) + b * a.out_s_seq + int64_t(h * g + q0 + head) * a.out_s_head;
+  const int vecs = D / 4;                              // (at most 64)
   if (units == 0) {
-    for (int u = tid; u < work; u += kTeam)
-      *reinterpret_cast<uint2*>(out + (u / vecs) * a.out_s_head + (u % vecs) * 4) = make_uint2(0, 0);
+    for (int v = tid; v < vecs; v += kTeam) *reinterpret_cast<uint2*>(out + v * 4) = make_uint2(0, 0);
     return;
   }
-  const int64_t per_warp = quotient(total + plan.warps - 1, plan.warps), per_cta = per_warp * kWarps;
-  const int64_t begin = before + int64_t(seg) * units, end = begin + units;
+  if constexpr (kTeam == 32) {
+    begin = plan.seg_begin[segment];
+    per_warp = plan.seg_begin[int64_t(a.batch) * per_row];
+    if (begin < 0) return;
+  }
+  const int64_t end = begin + units, per_cta = per_warp * kWarps;
   const int w0 = int(quotient(begin + kSetup, per_warp)), w1 = int(quotient(end - 1, per_warp));
-  if (w0 == w1) return;                             // stored by its warp
+  if (w0 == w1) return;                                // stored by its warp
   // its parts: warps w0 .., whole CTAs c0 .. c1 - 1, warps .. w1
   const int c0 = int(quotient(begin + kSetup + per_cta - 1, per_cta)), c1 = int(quotient(end, per_cta));
   const int n2 = max(c1 - c0, 0);
@@ -757,30 +769,42 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(KittyKv8AttentionA
   const int parts = n2 ? n1 + n2 + (w1 - c1 * kWarps + 1) : n1;
   auto place = [&](int i) {
     const int w = i < n1 ? w0 + i : i < n1 + n2 ? (c0 + i - n1) * kWarps : c1 * kWarps + (i - n1 - n2);
-    return (2 * int64_t(w) + (begin > w * per_warp)) * plan.pass_heads + first_head;
+    return (2 * int64_t(w) + (begin > w * per_warp)) * plan.pass_heads + head;
   };
-  const int groups = kTeam == 32 ? 1 : kTeam / vecs;  // (vecs <= 64)
-  for (int u0 = 0; u0 < work; u0 += kTeam) {        // (a CTA's team has one round: work == vecs)
-    const int group = kTeam == 32 ? 0 : tid / vecs;
-    const int u = kTeam == 32 ? u0 + tid : tid - group * vecs;
-    const bool mine = u < work && group < groups;
-    const int qh = mine ? u / vecs : 0, v = mine ? u - qh * vecs : 0;
+  const int groups = kTeam == 32 ? 1 : kTeam / vecs;
+  for (int v0 = 0; v0 < vecs; v0 += kTeam) {           // (a second round: a warp and more than 128 channels)
+    const int group = kTeam == 32 ? 0 : tid / vecs, v = kTeam == 32 ? v0 + tid : tid - group * vecs;
+    const bool mine = v < vecs && group < groups;
     float top = -INFINITY, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (mine) {
-#pragma unroll 4
-      for (int i = group; i < parts; i += groups) top = fmaxf(top, plan.part_ml[(place(i) + qh) * 2]);
-      const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll 4
-      for (int i = group; i < parts; i += groups) {
-        const int64_t at = place(i) + qh;
-        const float k = ex2(plan.part_ml[at * 2] - ref);
-        const float4 p = *reinterpret_cast<const float4*>(plan.part_o + at * D + v * 4);
-        sum = fmaf(k, plan.part_ml[at * 2 + 1], sum);
-        acc.x = fmaf(k, p.x, acc.x);
-        acc.y = fmaf(k, p.y, acc.y);
-        acc.z = fmaf(k, p.z, acc.z);
-        acc.w = fmaf(k, p.w, acc.w);
+    for (int i0 = group; mine && i0 < parts; i0 += groups * kBatch) {
+      float2 ml[kBatch];
+      float4 p[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int i = i0 + k * groups;
+        ml[k] = make_float2(-INFINITY, 0.f);
+        p[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < parts) {
+          const int64_t at = place(i);
+          ml[k] = *reinterpret_cast<const float2*>(plan.part_ml + at * 2);
+          p[k] = *reinterpret_cast<const float4*>(plan.part_o + at * D + v * 4);
+        }
+      }
+      const float old = top;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) top = fmaxf(top, ml[k].x);
+      const float ref = top == -INFINITY ? 0.f : top, f0 = ex2(old - ref);
+      sum *= f0;
+      acc = make_float4(acc.x * f0, acc.y * f0, acc.z * f0, acc.w * f0);
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const float f = ex2(ml[k].x - ref);
+        sum = fmaf(f, ml[k].y, sum);
+        acc.x = fmaf(f, p[k].x, acc.x);
+        acc.y = fmaf(f, p[k].y, acc.y);
+        acc.z = fmaf(f, p[k].z, acc.z);
+        acc.w = fmaf(f, p[k].w, acc.w);
       }
     }
     if constexpr (kTeam != 32) {
@@ -789,14 +813,14 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(KittyKv8AttentionA
       s_m[tid] = top;
       __syncthreads();
       if (mine && group == 0) {
-        for (int k = 1; k < groups; ++k) top = fmaxf(top, s_m[k * vecs + u]);
+        for (int k = 1; k < groups; ++k) top = fmaxf(top, s_m[k * vecs + v]);
         const float ref = top == -INFINITY ? 0.f : top;
         acc = make_float4(0.f, 0.f, 0.f, 0.f);
         sum = 0.f;
         for (int k = 0; k < groups; ++k) {
-          const float f = ex2(s_m[k * vecs + u] - ref);
-          const float4 p = s_sum[k * vecs + u];
-          sum = fmaf(f, s_l[k * vecs + u], sum);
+          const float f = ex2(s_m[k * vecs + v] - ref);
+          const float4 p = s_sum[k * vecs + v];
+          sum = fmaf(f, s_l[k * vecs + v], sum);
           acc.x = fmaf(f, p.x, acc.x);
           acc.y = fmaf(f, p.y, acc.y);
           acc.z = fmaf(f, p.z, acc.z);
@@ -806,7 +830,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(KittyKv8AttentionA
     }
     if (mine && group == 0) {
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      *reinterpret_cast<uint2*>(out + qh * a.out_s_head + v * 4) =
+      *reinterpret_cast<uint2*>(out + v * 4) =
           make_uint2(dev::from_f2<kBf16>(acc.x * inv, acc.y * inv), dev::from_f2<kBf16>(acc.z * inv, acc.w * inv));
     }
   }
@@ -844,33 +868,42 @@ int resident() {
   return known;
 }
 
+// The workspace: the segments' begins and the slice's units, the parts' maxima and sums, and
+// their outputs, each from a 256-byte boundary.  Returns its bytes.
+size_t lay_out(Plan& plan, const KittyKv8AttentionArgs& a, uint8_t* base) {
+  const auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  const size_t segments = size_t(a.batch) * a.cache.num_heads * plan.passes;
+  const size_t parts = size_t(2) * plan.warps * plan.pass_heads;
+  const size_t begins = up((segments + 1) * 8), ml = up(parts * 8);
+  plan.seg_begin = reinterpret_cast<int64_t*>(base);
+  plan.part_ml = reinterpret_cast<float*>(base + begins);
+  plan.part_o = reinterpret_cast<float*>(base + begins + ml);
+  return begins + ml + parts * a.cache.head_dim * 4;
+}
+
 template <int kDim, int kNT, bool kWhole, bool kBf16, int kCode>
-int launch(const KittyKv8AttentionArgs& a, Plan plan, uint32_t* err, cudaStream_t s, int* warps) {
+int launch(const KittyKv8AttentionArgs& a, Plan plan, uint32_t* err, cudaStream_t s, size_t* bytes) {
   const int grid = sm_count() * resident<kDim, kNT, kWhole, kBf16, kCode>();
   plan.warps = grid * kWarps;
-  if (warps) { *warps = plan.warps; return KITTY_OK; }
-  const size_t parts = size_t(2) * plan.warps * plan.pass_heads;
-  const size_t ml = (parts * 2 * 4 + 255) / 256 * 256;
-  if (a.workspace_bytes < ml + parts * a.cache.head_dim * 4)
+  const size_t need = lay_out(plan, a, static_cast<uint8_t*>(a.workspace));
+  if (bytes) { *bytes = need; return KITTY_OK; }
+  if (a.workspace_bytes < need)
     return fail(KITTY_ERR_WORKSPACE, "kv8_attention", "workspace smaller than kitty_kv8_attention_workspace_size()");
-  plan.part_ml = static_cast<float*>(a.workspace);
-  plan.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + ml);
   attention_kernel<kDim, kNT, kWhole, kBf16, kCode><<<grid, kWarps * 32, 0, s>>>(a, plan, err);
   const int rc = check_launch("kv8_attention");
   if (rc != KITTY_OK) return rc;
   constexpr int kTile = kDim == 256 ? 16 : 32;
   // Few segments are shared by many warps each, many segments are mostly one warp's own.
-  const unsigned segments = unsigned(a.batch) * a.cache.num_heads * plan.passes;
+  const unsigned segments = unsigned(a.batch) * a.cache.num_heads * plan.passes, teams = segments * plan.pass_heads;
   const unsigned per = kMergeThreads / 32;
-  const cudaError_t e =
-      segments < unsigned(plan.warps) / 4
-          ? launch_merge<kTile, kBf16, kMergeThreads>(a, plan, dim3(segments, unsigned(plan.pass_heads)), s)
-          : launch_merge<kTile, kBf16, 32>(a, plan, dim3((segments + per - 1) / per), s);
+  const cudaError_t e = segments < unsigned(plan.warps) / 4
+                            ? launch_merge<kTile, kBf16, kMergeThreads>(a, plan, dim3(teams), s)
+                            : launch_merge<kTile, kBf16, 32>(a, plan, dim3((teams + per - 1) / per), s);
   return e == cudaSuccess ? KITTY_OK : fail(KITTY_ERR_CUDA, "kv8_attention (merge)", cudaGetErrorString(e));
 }
 
 template <int kDim, bool kWhole, bool kBf16, int kCode>
-int launch_heads(const KittyKv8AttentionArgs& a, uint32_t* err, cudaStream_t s, int* warps, int* pass_heads) {
+int launch_heads(const KittyKv8AttentionArgs& a, uint32_t* err, cudaStream_t s, size_t* bytes) {
   // Query heads of a KV head in passes of 8 or 16: 16 columns share every conversion of
   // a code, but at 256 channels their outputs would not fit the registers.
   const int g = a.num_q_heads / a.cache.num_heads;
@@ -879,30 +912,29 @@ int launch_heads(const KittyKv8AttentionArgs& a, uint32_t* err, cudaStream_t s, 
   const int most = kTwo && g > 8 ? 16 : 8;
   plan.passes = (g + most - 1) / most;
   plan.pass_heads = (g + plan.passes - 1) / plan.passes;
-  if (pass_heads) *pass_heads = plan.pass_heads;
   if constexpr (kTwo) {
-    if (plan.pass_heads > 8) return launch<kDim, 2, kWhole, kBf16, kCode>(a, plan, err, s, warps);
+    if (plan.pass_heads > 8) return launch<kDim, 2, kWhole, kBf16, kCode>(a, plan, err, s, bytes);
   }
-  return launch<kDim, 1, kWhole, kBf16, kCode>(a, plan, err, s, warps);
+  return launch<kDim, 1, kWhole, kBf16, kCode>(a, plan, err, s, bytes);
 }
 
 template <bool kBf16, int kCode>
-int launch_dim(const KittyKv8AttentionArgs& a, uint32_t* err, cudaStream_t s, int* warps, int* ph) {
+int launch_dim(const KittyKv8AttentionArgs& a, uint32_t* err, cudaStream_t s, size_t* bytes) {
   const int D = a.cache.head_dim;
-  if (D == 64) return launch_heads<64, true, kBf16, kCode>(a, err, s, warps, ph);
-  if (D < 64) return launch_heads<64, false, kBf16, kCode>(a, err, s, warps, ph);
-  if (D == 128) return launch_heads<128, true, kBf16, kCode>(a, err, s, warps, ph);
-  if (D < 128) return launch_heads<128, false, kBf16, kCode>(a, err, s, warps, ph);
-  if (D == 256) return launch_heads<256, true, kBf16, kCode>(a, err, s, warps, ph);
-  return launch_heads<256, false, kBf16, kCode>(a, err, s, warps, ph);
+  if (D == 64) return launch_heads<64, true, kBf16, kCode>(a, err, s, bytes);
+  if (D < 64) return launch_heads<64, false, kBf16, kCode>(a, err, s, bytes);
+  if (D == 128) return launch_heads<128, true, kBf16, kCode>(a, err, s, bytes);
+  if (D < 128) return launch_heads<128, false, kBf16, kCode>(a, err, s, bytes);
+  if (D == 256) return launch_heads<256, true, kBf16, kCode>(a, err, s, bytes);
+  return launch_heads<256, false, kBf16, kCode>(a, err, s, bytes);
 }
 
-int dispatch(const KittyKv8AttentionArgs& a, uint32_t* err, cudaStream_t s, int* warps, int* ph) {
+int dispatch(const KittyKv8AttentionArgs& a, uint32_t* err, cudaStream_t s, size_t* bytes) {
   if (a.cache.dtype == KITTY_KV8_BF16)
-    return a.cache.code == KITTY_KV8_E4M3 ? launch_dim<true, KITTY_KV8_E4M3>(a, err, s, warps, ph)
-                                          : launch_dim<true, KITTY_KV8_INT8>(a, err, s, warps, ph);
-  return a.cache.code == KITTY_KV8_E4M3 ? launch_dim<false, KITTY_KV8_E4M3>(a, err, s, warps, ph)
-                                        : launch_dim<false, KITTY_KV8_INT8>(a, err, s, warps, ph);
+    return a.cache.code == KITTY_KV8_E4M3 ? launch_dim<true, KITTY_KV8_E4M3>(a, err, s, bytes)
+                                          : launch_dim<true, KITTY_KV8_INT8>(a, err, s, bytes);
+  return a.cache.code == KITTY_KV8_E4M3 ? launch_dim<false, KITTY_KV8_E4M3>(a, err, s, bytes)
+                                        : launch_dim<false, KITTY_KV8_INT8>(a, err, s, bytes);
 }
 
 int check_attention(const KittyKv8AttentionArgs* a, const char* what) {
@@ -914,8 +946,8 @@ int check_attention(const KittyKv8AttentionArgs* a, const char* what) {
     return fail(KITTY_ERR_INVALID_ARGUMENT, what, "num_q_heads must be a multiple of num_heads");
   if (!a->seq_map && a->batch > a->cache.slots)
     return fail(KITTY_ERR_INVALID_ARGUMENT, what, "more queries than slots");
-  if (int64_t(a->batch) * a->num_q_heads > 0x7fffffffLL)
-    return fail(KITTY_ERR_UNSUPPORTED, what, "batch * num_q_heads must fit 31 bits");
+  if (int64_t(a->batch) * a->num_q_heads > 0x3fffffffLL)   // (passes round a KV head's query heads up, to less than twice)
+    return fail(KITTY_ERR_UNSUPPORTED, what, "batch * num_q_heads must fit 30 bits");
   return KITTY_OK;
 }
 
@@ -929,11 +961,7 @@ extern "C" int kitty_kv8_attention_workspace_size(const KittyKv8AttentionArgs* a
   const int rc = check_attention(a, what);
   if (rc != KITTY_OK) return rc;
   if (!bytes) return fail(KITTY_ERR_INVALID_ARGUMENT, what, "bytes is NULL");
-  int warps = 0, ph = 0;
-  dispatch(*a, nullptr, nullptr, &warps, &ph);
-  const size_t parts = size_t(2) * warps * ph;
-  *bytes = (parts * 2 * 4 + 255) / 256 * 256 + parts * a->cache.head_dim * 4;
-  return KITTY_OK;
+  return dispatch(*a, nullptr, nullptr, bytes);
 }
 
 extern "C" int kitty_kv8_attention(const KittyKv8AttentionArgs* a, void* stream) {
@@ -950,5 +978,5 @@ extern "C" int kitty_kv8_attention(const KittyKv8AttentionArgs* a, void* stream)
     return fail(KITTY_ERR_WORKSPACE, what, "workspace missing or not 16-byte aligned");
   uint32_t* err = error_word();
   if (!err) return fail(KITTY_ERR_CUDA, what, "no CUDA device");
-  return dispatch(*a, err, as_stream(stream), nullptr, nullptr);
+  return dispatch(*a, err, as_stream(stream), nullptr);
 }
