@@ -1,30 +1,32 @@
 // Reading the cache back to 16-bit rows.
 //
-// A CTA takes kRowsPerCta output rows (tokens, all heads).  Its first warp finds each
-// row's slot and page by a search of the row offsets and leaves them in shared memory;
-// then every thread turns eight codes of keys and of values (8 bytes each) into 16-byte
-// stores, contiguous over the row.  Bound by HBM: 1 byte read and 2 written a value.
+// A CTA takes kRows output rows (tokens, all heads).  Its first warp finds each row's slot
+// and page by a search of the row offsets and leaves them in shared memory; then every
+// thread turns eight codes of keys and of values (8 bytes each) into 16-byte stores,
+// contiguous over the row, at the same place of one row after another.  Bound by HBM: 1
+// byte read and 2 written a value.
 #include "kv8_common.cuh"
 
 namespace kitty8 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRowsPerCta = 32;
-constexpr int kUnroll = 4;
+constexpr int kUnroll = 4;      // rows whose loads a thread has in flight
+
+constexpr int64_t kManyValues = 5 * 32 * 1024;   // keys for each SM: five CTAs of 32 rows of 1024
 
 struct RowAt {
   int64_t base;        // element offset of (row, head 0, channel 0) in the pools or the tails
   int32_t page;        // -1: a tail row, -2: nothing to do
 };
 
-template <bool kBf16, int kCode>
+template <bool kBf16, int kCode, int kRows>
 __global__ void __launch_bounds__(kThreads) read_kernel(KittyKv8ReadArgs a, uint32_t* err) {
-  __shared__ RowAt s_row[kRowsPerCta];
+  __shared__ RowAt s_row[kRows];
   const KittyKv8Cache& c = a.cache;
   const int G = c.page_size, D = c.head_dim, H = c.num_heads;
-  const int64_t r0 = int64_t(blockIdx.x) * kRowsPerCta;
-  const int count = int(min(int64_t(kRowsPerCta), a.rows - r0));
+  const int64_t r0 = int64_t(blockIdx.x) * kRows;
+  const int count = int(min(int64_t(kRows), a.rows - r0));
   if (int(threadIdx.x) < count) {
     const int r = int(r0) + threadIdx.x;
     int lo = 0, hi = a.n + 1;            // how many offsets are <= r (any contents end within the bounds)
@@ -65,46 +67,50 @@ __global__ void __launch_bounds__(kThreads) read_kernel(KittyKv8ReadArgs a, uint
     s_row[threadIdx.x] = at;
   }
   __syncthreads();
-  const int per = D / 8, vecs = H * per, units = count * vecs;
+  const int per = D / 8, vecs = H * per;
   const int64_t s_head = int64_t(G) * D;
-  uint4* const out[2] = {static_cast<uint4*>(a.key) + r0 * vecs, static_cast<uint4*>(a.value) + r0 * vecs};
-  const uint8_t* const codes[2] = {static_cast<const uint8_t*>(c.key_codes), static_cast<const uint8_t*>(c.value_codes)};
-  const uint16_t* const tails[2] = {static_cast<const uint16_t*>(c.tail_k), static_cast<const uint16_t*>(c.tail_v)};
-  const float* const scales[2] = {c.key_scale, c.value_scale};
-  for (int u0 = threadIdx.x; u0 < units; u0 += kThreads * kUnroll) {
-    uint2 w[kUnroll][2];
-    float sc[kUnroll][2];
-    int page[kUnroll];
+  // the threads lie over as many rows as fit, or several times over one
+  const int at_once = max(1, kThreads / vecs), row0 = vecs <= kThreads ? threadIdx.x / vecs : 0;
+  if (row0 >= at_once) return;
+  for (int v = vecs <= kThreads ? threadIdx.x - row0 * vecs : threadIdx.x; v < vecs; v += kThreads) {
+    const int h = v / per;
+    const int64_t place = h * s_head + (v - h * per) * 8;
+    for (int r = row0; r < count; r += at_once * kUnroll) {
+      uint2 w[kUnroll][2];
+      float sc[kUnroll][2];
+      int page[kUnroll];
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) {
-      const int u = u0 + k * kThreads;
-      page[k] = -2;
-      if (u < units) {
-        const int row = u / vecs, v = u - row * vecs, h = v / per, d = v - h * per;
-        const RowAt at = s_row[row];
-        page[k] = at.page;
-        const int64_t off = at.base + h * s_head + d * 8;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
+      for (int k = 0; k < kUnroll; ++k) {
+        const int row = r + k * at_once;
+        page[k] = -2;
+        if (row < count) {
+          const RowAt at = s_row[row];
+          const int64_t off = at.base + place, to = (r0 + row) * vecs + v;
+          page[k] = at.page;
           if (at.page >= 0) {
-            w[k][x] = __ldg(reinterpret_cast<const uint2*>(codes[x] + off));
-            sc[k][x] = __ldg(scales[x] + int64_t(at.page) * H + h);
+            const int64_t scale = int64_t(at.page) * H + h;
+            w[k][0] = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(c.key_codes) + off));
+            w[k][1] = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(c.value_codes) + off));
+            sc[k][0] = __ldg(c.key_scale + scale);
+            sc[k][1] = __ldg(c.value_scale + scale);
           } else if (at.page == -1) {
-            out[x][u] = *reinterpret_cast<const uint4*>(tails[x] + off);
+            static_cast<uint4*>(a.key)[to] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.tail_k) + off);
+            static_cast<uint4*>(a.value)[to] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.tail_v) + off);
           }
         }
       }
-    }
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) {
-      if (page[k] < 0) continue;
-      const int u = u0 + k * kThreads;
+      for (int k = 0; k < kUnroll; ++k) {
+        if (page[k] < 0) continue;
+        const int64_t to = (r0 + r + k * at_once) * vecs + v;
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const float4 p = dev::decode4<kCode>(w[k][x].x), q = dev::decode4<kCode>(w[k][x].y);
-        const float s = sc[k][x];
-        out[x][u] = make_uint4(dev::from_f2<kBf16>(p.x * s, p.y * s), dev::from_f2<kBf16>(p.z * s, p.w * s),
-                               dev::from_f2<kBf16>(q.x * s, q.y * s), dev::from_f2<kBf16>(q.z * s, q.w * s));
+        for (int x = 0; x < 2; ++x) {
+          const float4 p = dev::decode4<kCode>(w[k][x].x), q = dev::decode4<kCode>(w[k][x].y);
+          const float s = sc[k][x];
+          static_cast<uint4*>(x ? a.value : a.key)[to] =
+              make_uint4(dev::from_f2<kBf16>(p.x * s, p.y * s), dev::from_f2<kBf16>(p.z * s, p.w * s),
+                         dev::from_f2<kBf16>(q.x * s, q.y * s), dev::from_f2<kBf16>(q.z * s, q.w * s));
+        }
       }
     }
   }
@@ -112,8 +118,11 @@ __global__ void __launch_bounds__(kThreads) read_kernel(KittyKv8ReadArgs a, uint
 
 template <bool kBf16, int kCode>
 int launch(const KittyKv8ReadArgs& a, uint32_t* err, cudaStream_t s) {
-  const unsigned grid = unsigned((int64_t(a.rows) + kRowsPerCta - 1) / kRowsPerCta);
-  read_kernel<kBf16, kCode><<<grid, kThreads, 0, s>>>(a, err);
+  // Many rows: 32 a CTA, which finds their pages once.  Few: 8, so that every SM has some.
+  if (int64_t(a.rows) * a.cache.num_heads * a.cache.head_dim > kManyValues * sm_count())
+    read_kernel<kBf16, kCode, 32><<<unsigned((int64_t(a.rows) + 31) / 32), kThreads, 0, s>>>(a, err);
+  else
+    read_kernel<kBf16, kCode, 8><<<unsigned((int64_t(a.rows) + 7) / 8), kThreads, 0, s>>>(a, err);
   return check_launch("kv8_read");
 }
 

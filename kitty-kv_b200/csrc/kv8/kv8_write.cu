@@ -18,6 +18,9 @@ namespace kitty8 {
 namespace {
 
 constexpr int kHeld = 4;        // 16-byte vectors a thread holds in registers for each of key and value
+constexpr int kThreads = 256;
+constexpr int kMinCtas = 4;     // resident on an SM: 78K ragged rows take 109 us at 2, 88 at 3, 77 at 4, 96 at 5
+constexpr int kStepEntries = 8; // entries of a decode step whose blocks one CTA looks after
 
 // Source rows of a block: the first `have` from the tail, the others from the call's rows.
 struct Rows {
@@ -27,7 +30,14 @@ struct Rows {
   int have;
 };
 
-__device__ __forceinline__ uint4 load_vec(const Rows& r, int D, int t, int c) {
+// 16-byte vectors of a row: known when compiled for the usual head sizes, so that finding
+// a vector's row takes a shift and not a division.
+template <int kPer>
+__device__ __forceinline__ int vecs_of_row(int D) { return kPer ? kPer : D / 8; }
+
+template <int kPer>
+__device__ __forceinline__ uint4 load_vec(const Rows& r, int D, int v) {
+  const int per = vecs_of_row<kPer>(D), t = v / per, c = v - t * per;
   const uint16_t* p = t < r.have ? r.tail + t * D : r.fresh + int64_t(t - r.have) * r.s_row;
   return *(reinterpret_cast<const uint4*>(p) + c);
 }
@@ -48,12 +58,24 @@ __device__ __forceinline__ uint2 encode_vec(const uint4& v, float r) {
                     dev::encode4<kCode>(c.x * r, c.y * r, d.x * r, d.y * r));
 }
 
-// Quantise one block of keys and one of values by the whole CTA.
-template <bool kBf16, int kCode, int kThreads>
-__device__ __forceinline__ void quantise_block(const Rows (&src)[2], uint8_t* const (&codes)[2], float* const (&scale)[2], int G, int D,
-                               uint32_t (*s_top)[kThreads / 32]) {
+// The page of block b of a slot; -1 (and flagged) if the cache has none.
+__device__ __forceinline__ int page_of(const KittyKv8Cache& c, int slot, int b, uint32_t* err) {
+  int page = -1;
+  if (b < c.max_pages) page = c.block_table[int64_t(slot) * c.bt_s_slot + b];
+  if (page < 0 || page >= c.pages) {
+    if (threadIdx.x == 0) dev::flag(err, kErrPage);
+    return -1;
+  }
+  return page;
+}
+
+// Quantise block `block` of a slot's head h from its key and value rows, by the whole CTA.
+// The rows are asked for first and the page looked up while they are on their way.
+template <bool kBf16, int kCode, int kPer>
+__device__ __forceinline__ void quantise_block(const KittyKv8Cache& c, int slot, int block, int h, const Rows (&src)[2],
+                                               uint32_t (*s_top)[kThreads / 32], uint32_t* err) {
   constexpr float kQ = kCode == KITTY_KV8_E4M3 ? 448.f : 127.f;
-  const int tid = threadIdx.x, per = D / 8, vecs = G * per;
+  const int G = c.page_size, D = c.head_dim, tid = threadIdx.x, vecs = G * vecs_of_row<kPer>(D);
   uint4 held[2][kHeld];
   uint32_t top[2] = {0u, 0u};
 #pragma unroll
@@ -61,21 +83,23 @@ __device__ __forceinline__ void quantise_block(const Rows (&src)[2], uint8_t* co
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
       const int v = tid + i * kThreads;
-      held[x][i] = v < vecs ? load_vec(src[x], D, v / per, v % per) : make_uint4(0, 0, 0, 0);
+      held[x][i] = v < vecs ? load_vec<kPer>(src[x], D, v) : make_uint4(0, 0, 0, 0);
     }
   }
+  const int page = page_of(c, slot, block, err);
+  if (page < 0) return;
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) top[x] = top_of<kBf16>(held[x][i], top[x]);
-    for (int v = tid + kHeld * kThreads; v < vecs; v += kThreads)
-      top[x] = top_of<kBf16>(load_vec(src[x], D, v / per, v % per), top[x]);
+    for (int v = tid + kHeld * kThreads; v < vecs; v += kThreads) top[x] = top_of<kBf16>(load_vec<kPer>(src[x], D, v), top[x]);
     top[x] = dev::max2<kBf16>(top[x], (top[x] >> 16) | (top[x] << 16));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top[x] = dev::max2<kBf16>(top[x], __shfl_xor_sync(0xffffffffu, top[x], o));
     if ((tid & 31) == 0) s_top[x][tid >> 5] = top[x];
   }
   __syncthreads();
+  const int64_t at = int64_t(page) * c.num_heads + h;
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     uint32_t m = s_top[x][0];
@@ -84,14 +108,15 @@ __device__ __forceinline__ void quantise_block(const Rows (&src)[2], uint8_t* co
     const float a = dev::to_f2<kBf16>(m).x;
     const float top_f = a < 0x1p-100f ? 0x1p-100f : a;       // NaN stays
     const float r = __frcp_rn(top_f) * kQ;                   // each factor rounded once
-    if (tid == 0) *scale[x] = top_f * (1.f / kQ);
+    if (tid == 0) (x ? c.value_scale : c.key_scale)[at] = top_f * (1.f / kQ);
+    uint2* codes = reinterpret_cast<uint2*>(static_cast<uint8_t*>(x ? c.value_codes : c.key_codes) + at * G * D);
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
       const int v = tid + i * kThreads;
-      if (v < vecs) reinterpret_cast<uint2*>(codes[x])[v] = encode_vec<kBf16, kCode>(held[x][i], r);
+      if (v < vecs) codes[v] = encode_vec<kBf16, kCode>(held[x][i], r);
     }
     for (int v = tid + kHeld * kThreads; v < vecs; v += kThreads)
-      reinterpret_cast<uint2*>(codes[x])[v] = encode_vec<kBf16, kCode>(load_vec(src[x], D, v / per, v % per), r);
+      codes[v] = encode_vec<kBf16, kCode>(load_vec<kPer>(src[x], D, v), r);
   }
 }
 
@@ -116,85 +141,126 @@ __device__ __forceinline__ bool entry_of(const KittyKv8WriteArgs& a, int i, bool
   return bad == 0;
 }
 
-// The page of block b of a slot; -1 (and flagged) if the cache has none.
-__device__ __forceinline__ int page_of(const KittyKv8Cache& c, int slot, int b, uint32_t* err) {
-  int page = -1;
-  if (b < c.max_pages) page = c.block_table[int64_t(slot) * c.bt_s_slot + b];
-  if (page < 0 || page >= c.pages) {
-    if (threadIdx.x == 0) dev::flag(err, kErrPage);
-    return -1;
-  }
-  return page;
+__device__ __forceinline__ const uint16_t* row_of(const void* base, int64_t row, int64_t s_row, int64_t h, int64_t s_head) {
+  return static_cast<const uint16_t*>(base) + row * s_row + h * s_head;
 }
 
-template <bool kBf16, int kCode, int kThreads>
-__global__ void __launch_bounds__(kThreads) write_kernel(KittyKv8WriteArgs a, uint32_t* err) {
+// Ragged rows.  CTAs run over the heads first: those that are resident together read whole
+// rows of the tokens, and not one head's slice of many.
+template <bool kBf16, int kCode, int kPer>
+__global__ void __launch_bounds__(kThreads, kMinCtas) write_kernel(KittyKv8WriteArgs a, uint32_t* err) {
   __shared__ uint32_t s_top[2][kThreads / 32];
   const KittyKv8Cache& c = a.cache;
-  const int G = c.page_size, D = c.head_dim, h = blockIdx.y;
-  const int64_t block_elems = int64_t(G) * D;
+  const int G = c.page_size, D = c.head_dim;
+  const int item = blockIdx.x / c.num_heads, h = blockIdx.x - item * c.num_heads;
   int slot, o, len, cached;
-  int block, have, skip;        // the block to quantise: its tail rows, and the entry's rows before its first new row
-  bool whole;
-  const bool entry_cta = int(blockIdx.x) < a.n;
-  if (entry_cta) {
-    if (!entry_of(a, blockIdx.x, h == 0, err, slot, o, len, cached)) return;
-    block = cached / G;
-    have = cached % G;
-    skip = 0;
-    whole = have > 0 && have + len >= G;
+  if (item < a.n) {
+    if (!entry_of(a, item, h == 0, err, slot, o, len, cached)) return;
+    const int block = cached / G, have = cached - block * G;
+    const bool whole = have > 0 && have + len >= G;
+    // the rows that fill no block: behind the tail's, or from its first row if a block was completed
+    const int left = have + len < G ? len : int((int64_t(cached) + len) % G);
+    const int to = have + len < G ? have : 0, per = vecs_of_row<kPer>(D);
+    const int64_t tail = (int64_t(slot) * c.num_heads + h) * G * D;
+    uint16_t* const tail_k = static_cast<uint16_t*>(c.tail_k) + tail;
+    uint16_t* const tail_v = static_cast<uint16_t*>(c.tail_v) + tail;
+    if (whole) {
+      const Rows src[2] = {{tail_k, row_of(a.key, o, a.k_s_row, h, a.k_s_head), a.k_s_row, have},
+                           {tail_v, row_of(a.value, o, a.v_s_row, h, a.v_s_head), a.v_s_row, have}};
+      quantise_block<kBf16, kCode, kPer>(c, slot, block, h, src, s_top, err);
+      __syncthreads();   // every thread has read the tail rows of the block
+    }
+    for (int u = threadIdx.x; u < 2 * left * per; u += kThreads) {
+      const int x = u >= left * per, v = u - x * left * per, t = v / per, d = v - t * per;
+      const uint16_t* src = x ? row_of(a.value, o + len - left + t, a.v_s_row, h, a.v_s_head)
+                              : row_of(a.key, o + len - left + t, a.k_s_row, h, a.k_s_head);
+      reinterpret_cast<uint4*>((x ? tail_v : tail_k) + (to + t) * D)[d] = reinterpret_cast<const uint4*>(src)[d];
+    }
   } else {
-    const int64_t last = int64_t(int(blockIdx.x) - a.n) * G + G - 1;   // < rows by the grid's size
+    const int64_t last = int64_t(item - a.n) * G + G - 1;              // < rows by the grid's size
     const int i = dev::count_le(a.row_offsets, a.n + 1, int(last)) - 1;
     if (i < 0 || i >= a.n) return;                                     // rows behind the last entry
     if (!entry_of(a, i, false, err, slot, o, len, cached)) return;
     const int64_t local = last - o;
     if (local < 0 || local >= len) return;
-    block = int((cached + local) / G);
-    have = 0;
-    const int64_t first = int64_t(block) * G - cached;
-    whole = first >= 0 && first + G <= len;
-    if (!whole) return;
-    skip = int(first);
-  }
-  const int64_t tail = (int64_t(slot) * c.num_heads + h) * block_elems;
-  uint16_t* tails[2] = {static_cast<uint16_t*>(c.tail_k) + tail, static_cast<uint16_t*>(c.tail_v) + tail};
-  const int64_t s_row[2] = {a.k_s_row, a.v_s_row};
-  const uint16_t* rows[2] = {static_cast<const uint16_t*>(a.key) + int64_t(o) * a.k_s_row + h * a.k_s_head,
-                             static_cast<const uint16_t*>(a.value) + int64_t(o) * a.v_s_row + h * a.v_s_head};
-  if (whole) {
-    const int page = page_of(c, slot, block, err);
-    if (page >= 0) {
-      const int64_t at = int64_t(page) * c.num_heads + h;
-      const Rows src[2] = {{tails[0], rows[0] + skip * s_row[0], s_row[0], have},
-                           {tails[1], rows[1] + skip * s_row[1], s_row[1], have}};
-      uint8_t* const codes[2] = {static_cast<uint8_t*>(c.key_codes) + at * block_elems,
-                                 static_cast<uint8_t*>(c.value_codes) + at * block_elems};
-      float* const scale[2] = {c.key_scale + at, c.value_scale + at};
-      quantise_block<kBf16, kCode, kThreads>(src, codes, scale, G, D, s_top);
-    }
-  }
-  if (!entry_cta) return;
-  // the rows that fill no block: behind the tail's, or from its first row if a block was completed
-  const int left = have + len < G ? len : int((int64_t(cached) + len) % G);
-  const int to = have + len < G ? have : 0;
-  if (left == 0) return;
-  if (whole) __syncthreads();   // every thread has read the tail rows of the block
-  const int per = D / 8;
-  for (int u = threadIdx.x; u < 2 * left * per; u += kThreads) {
-    const int x = u >= left * per, v = u - x * left * per, t = v / per, d = v % per;
-    const uint16_t* src = x ? rows[1] + int64_t(len - left + t) * s_row[1] : rows[0] + int64_t(len - left + t) * s_row[0];
-    reinterpret_cast<uint4*>((x ? tails[1] : tails[0]) + (to + t) * D)[d] = reinterpret_cast<const uint4*>(src)[d];
+    const int block = int((cached + local) / G);
+    const int64_t first = int64_t(block) * G - cached;                 // the entry's row that the block begins with
+    if (first < 0 || first + G > len) return;
+    const Rows src[2] = {{nullptr, row_of(a.key, o + first, a.k_s_row, h, a.k_s_head), a.k_s_row, 0},
+                         {nullptr, row_of(a.value, o + first, a.v_s_row, h, a.v_s_head), a.v_s_row, 0}};
+    quantise_block<kBf16, kCode, kPer>(c, slot, block, h, src, s_top, err);
   }
 }
 
-template <bool kBf16, int kCode>
+// One row for each entry, a decode step.  The first CTAs look at one head of kStepEntries
+// entries and quantise the blocks that this row completes (one in G, when the lengths are
+// spread); the others copy an entry's row into the tails, all heads at once.  One CTA for
+// each entry and head took 10.4 us for 256 entries and 8 heads: 2048 CTAs, most of which
+// copy 512 bytes.
+template <bool kBf16, int kCode, int kPer>
+__global__ void __launch_bounds__(kThreads, kMinCtas) write_step_kernel(KittyKv8WriteArgs a, uint32_t* err) {
+  __shared__ uint32_t s_top[2][kThreads / 32];
+  const KittyKv8Cache& c = a.cache;
+  const int G = c.page_size, D = c.head_dim, H = c.num_heads, per = vecs_of_row<kPer>(D);
+  const int groups = (a.n + kStepEntries - 1) / kStepEntries;
+  int slot, o, len, cached;
+  if (int(blockIdx.x) < groups * H) {
+    const int group = blockIdx.x / H, h = blockIdx.x - group * H, lane = threadIdx.x & 31;
+    // every warp looks at the group's lengths, one a lane
+    const int i0 = group * kStepEntries;
+    bool full = false;
+    if (lane < kStepEntries && i0 + lane < a.n) {
+      const int s = a.seq_map ? a.seq_map[i0 + lane] : i0 + lane;
+      const int n = s >= 0 && s < c.slots ? c.lengths[s] : -1;
+      full = n >= 0 && n % G == G - 1;
+    }
+    for (uint32_t todo = __ballot_sync(0xffffffffu, full); todo; todo &= todo - 1) {
+      if (!entry_of(a, i0 + __ffs(todo) - 1, false, err, slot, o, len, cached)) continue;
+      const int64_t tail = (int64_t(slot) * H + h) * G * D;
+      const Rows src[2] = {{static_cast<const uint16_t*>(c.tail_k) + tail, row_of(a.key, o, a.k_s_row, h, a.k_s_head),
+                            a.k_s_row, G - 1},
+                           {static_cast<const uint16_t*>(c.tail_v) + tail, row_of(a.value, o, a.v_s_row, h, a.v_s_head),
+                            a.v_s_row, G - 1}};
+      quantise_block<kBf16, kCode, kPer>(c, slot, cached / G, h, src, s_top, err);
+      __syncthreads();   // s_top is used again
+    }
+    return;
+  }
+  const int i = blockIdx.x - groups * H, vecs = H * per;
+  auto source = [&](int u) {     // vector u of the entry's key row and then its value row
+    const int x = u >= vecs, v = u - x * vecs, h = v / per;
+    return *(reinterpret_cast<const uint4*>(x ? row_of(a.value, i, a.v_s_row, h, a.v_s_head)
+                                              : row_of(a.key, i, a.k_s_row, h, a.k_s_head)) + (v - h * per));
+  };
+  int u = threadIdx.x;
+  uint4 w = u < 2 * vecs ? source(u) : make_uint4(0, 0, 0, 0);     // on its way while the entry is looked up
+  if (!entry_of(a, i, true, err, slot, o, len, cached)) return;
+  const int row = cached % G;
+  if (row == G - 1) return;      // quantised with its block
+  for (; u < 2 * vecs; u += kThreads) {
+    if (u >= kThreads) w = source(u);
+    const int x = u >= vecs, v = u - x * vecs, h = v / per;
+    uint16_t* tail = static_cast<uint16_t*>(x ? c.tail_v : c.tail_k) + ((int64_t(slot) * H + h) * G + row) * D;
+    reinterpret_cast<uint4*>(tail)[v - h * per] = w;
+  }
+}
+
+template <bool kBf16, int kCode, int kPer>
 int launch(const KittyKv8WriteArgs& a, uint32_t* err, cudaStream_t s) {
-  const int64_t windows = a.row_offsets ? a.rows / a.cache.page_size : 0;
-  const dim3 grid(unsigned(a.n + windows), unsigned(a.cache.num_heads));
-  if (windows) write_kernel<kBf16, kCode, 256><<<grid, 256, 0, s>>>(a, err);
-  else write_kernel<kBf16, kCode, 128><<<grid, 128, 0, s>>>(a, err);   // mostly single rows: 2 D / 8 threads copy
+  const int64_t H = a.cache.num_heads;
+  const int64_t ctas = a.row_offsets ? (int64_t(a.n) + a.rows / a.cache.page_size) * H
+                                     : (int64_t(a.n) + kStepEntries - 1) / kStepEntries * H + a.n;
+  if (ctas > 0x7fffffff) return fail(KITTY_ERR_UNSUPPORTED, "kv8_write", "too many rows times heads for one launch");
+  if (a.row_offsets) write_kernel<kBf16, kCode, kPer><<<unsigned(ctas), kThreads, 0, s>>>(a, err);
+  else write_step_kernel<kBf16, kCode, kPer><<<unsigned(ctas), kThreads, 0, s>>>(a, err);
   return check_launch("kv8_write");
+}
+
+template <bool kBf16, int kCode>
+int launch_dim(const KittyKv8WriteArgs& a, uint32_t* err, cudaStream_t s) {
+  if (a.cache.head_dim == 64) return launch<kBf16, kCode, 8>(a, err, s);
+  if (a.cache.head_dim == 128) return launch<kBf16, kCode, 16>(a, err, s);
+  return launch<kBf16, kCode, 0>(a, err, s);
 }
 
 }  // namespace
@@ -222,8 +288,8 @@ extern "C" int kitty_kv8_write(const KittyKv8WriteArgs* a, void* stream) {
   if (!err) return fail(KITTY_ERR_CUDA, what, "no CUDA device");
   cudaStream_t s = as_stream(stream);
   if (a->cache.dtype == KITTY_KV8_BF16)
-    return a->cache.code == KITTY_KV8_E4M3 ? launch<true, KITTY_KV8_E4M3>(*a, err, s)
-                                           : launch<true, KITTY_KV8_INT8>(*a, err, s);
-  return a->cache.code == KITTY_KV8_E4M3 ? launch<false, KITTY_KV8_E4M3>(*a, err, s)
-                                         : launch<false, KITTY_KV8_INT8>(*a, err, s);
+    return a->cache.code == KITTY_KV8_E4M3 ? launch_dim<true, KITTY_KV8_E4M3>(*a, err, s)
+                                           : launch_dim<true, KITTY_KV8_INT8>(*a, err, s);
+  return a->cache.code == KITTY_KV8_E4M3 ? launch_dim<false, KITTY_KV8_E4M3>(*a, err, s)
+                                         : launch_dim<false, KITTY_KV8_INT8>(*a, err, s);
 }
