@@ -4,21 +4,31 @@
 // that rotates pairs 8j .. 8j+7 has all sixteen values of those pairs in registers
 // (two 16-byte loads), so the rotation needs no exchange and the mean of squares one
 // butterfly over the group.  A warp keeps its token's cosines and sines over up to
-// kPasses rows per group and issues the loads of all of them first.
+// kPasses rows per group.  It is bound by HBM, 2 bytes read and 2 written a channel, and
+// what is in flight counts: a warp's next token is copied to shared memory while this one
+// is worked on.  Every thread reads back only what it copied itself, so nothing is
+// synchronised.
 #include "kv8_common.cuh"
 
 namespace kitty8 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPasses = 4;     // rows per lane group and token: the table values are read once for them
+constexpr int kCtas = 2;       // resident on an SM
 
 struct RopeShape {
   int q_chunks, chunks;        // warps per token: ceil(heads / rows of a warp), queries first
 };
 
-template <bool kBf16, int kLanes, bool kInter>
-__global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(KittyQkNormRopeArgs a, RopeShape sh, uint32_t* err) {
+__device__ __forceinline__ void copy_async(uint4* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+               :: "r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(src) : "memory");
+}
+
+// kPasses: rows per lane group and token, which share the table values; kStages: tokens of
+// a warp in flight in shared memory, 0: no stage, the rows go to registers.
+template <bool kBf16, int kLanes, bool kInter, int kPasses, int kStages>
+__global__ void __launch_bounds__(kThreads, kCtas) qk_norm_rope_kernel(KittyQkNormRopeArgs a, RopeShape sh, uint32_t* err) {
   constexpr int kRows = 32 / kLanes;                       // rows that a warp holds at once
   const int lane = threadIdx.x & 31, j = lane % kLanes;
   const int64_t warps = int64_t(gridDim.x) * (kThreads / 32) / sh.chunks * sh.chunks;
@@ -55,25 +65,50 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(KittyQkNormRopeA
     }
   }
   const float inv_d = 1.f / float(D);
-  for (int64_t t = gw / sh.chunks; t < a.rows; t += warps / sh.chunks) {
-    const int64_t pos = a.positions64 ? static_cast<const int64_t*>(a.positions)[t]
-                                      : int64_t(static_cast<const int32_t*>(a.positions)[t]);
+  // [stage][warp][pass][half][lane]
+  extern __shared__ uint4 s_x[];
+  uint4* const mine = s_x + (threadIdx.x >> 5) * (kPasses * 2 * 32) + lane;
+  [[maybe_unused]] constexpr int kStage = (kThreads / 32) * kPasses * 2 * 32;
+  const int64_t step = warps / sh.chunks;
+  uint4 direct[kStages ? 1 : kPasses * 2];
+  auto fetch = [&](int64_t t, int stage) {
+    if (kStages == 0 || (t < a.rows && active)) {
+#pragma unroll
+      for (int p = 0; p < kPasses; ++p) {
+        const int h = h0 + p * kRows;
+        const uint16_t* r = in + t * s_row + h * s_head;
+        if constexpr (kStages > 0) {
+          if (h < heads) {
+            copy_async(mine + stage * kStage + p * 64, r + c0);
+            copy_async(mine + stage * kStage + p * 64 + 32, r + c1);
+          }
+        } else {
+          const bool there = active && h < heads;
+          direct[2 * p] = there ? *reinterpret_cast<const uint4*>(r + c0) : make_uint4(0, 0, 0, 0);
+          direct[2 * p + 1] = there ? *reinterpret_cast<const uint4*>(r + c1) : make_uint4(0, 0, 0, 0);
+        }
+      }
+    }
+    if constexpr (kStages > 0) asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto position = [&](int64_t t) {
+    return t >= a.rows ? int64_t(-1)
+           : a.positions64 ? static_cast<const int64_t*>(a.positions)[t]
+                           : int64_t(static_cast<const int32_t*>(a.positions)[t]);
+  };
+  int64_t t = gw / sh.chunks;
+#pragma unroll
+  for (int i = 0; i + 1 < kStages; ++i) fetch(t + i * step, i);
+  int64_t next = position(t);                               // read a token ahead: the table waits for it
+  for (int stage = 0; t < a.rows; t += step, stage = stage + 1 == kStages ? 0 : stage + 1) {
+    const int64_t pos = next;
+    next = position(t + step);
+    if constexpr (kStages > 0) fetch(t + (kStages - 1) * step, stage == 0 ? kStages - 1 : stage - 1);
+    else fetch(t, 0);
     if (pos < 0) continue;                                  // a padding row
     if (pos >= a.table_rows) {
       if (lane == 0) dev::flag(err, kErrPosition);
       continue;
-    }
-    uint4 x[kPasses][2];
-#pragma unroll
-    for (int p = 0; p < kPasses; ++p) {
-      const int h = h0 + p * kRows;
-      if (active && h < heads) {
-        const uint16_t* r = in + t * s_row + h * s_head;
-        x[p][0] = *reinterpret_cast<const uint4*>(r + c0);
-        x[p][1] = *reinterpret_cast<const uint4*>(r + c1);
-      } else {
-        x[p][0] = x[p][1] = make_uint4(0, 0, 0, 0);
-      }
     }
     float cs[8], sn[8];
     if (rotates) {
@@ -86,13 +121,19 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(KittyQkNormRopeA
         sn[4 * i] = v.x; sn[4 * i + 1] = v.y; sn[4 * i + 2] = v.z; sn[4 * i + 3] = v.w;
       }
     }
+    if constexpr (kStages > 0) asm volatile("cp.async.wait_group %0;" :: "n"(kStages - 1) : "memory");
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
       const int h = h0 + p * kRows;
       float y[16];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const uint32_t u[4] = {x[p][half].x, x[p][half].y, x[p][half].z, x[p][half].w};
+        uint4 x;
+        if constexpr (kStages > 0)
+          x = active && h < heads ? mine[stage * kStage + p * 64 + half * 32] : make_uint4(0, 0, 0, 0);
+        else
+          x = direct[2 * p + half];
+        const uint32_t u[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float2 f = dev::to_f2<kBf16>(u[i]);
@@ -133,7 +174,7 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(KittyQkNormRopeA
   }
 }
 
-template <bool kBf16, int kLanes>
+template <bool kBf16, int kLanes, int kPasses, int kStages>
 int launch(const KittyQkNormRopeArgs& a, uint32_t* err, cudaStream_t s) {
   constexpr int kHeads = 32 / kLanes * kPasses;
   RopeShape sh;
@@ -141,18 +182,34 @@ int launch(const KittyQkNormRopeArgs& a, uint32_t* err, cudaStream_t s) {
   sh.chunks = sh.q_chunks + (a.num_k_heads + kHeads - 1) / kHeads;
   const int64_t warps = int64_t(a.rows) * sh.chunks, per = kThreads / 32;
   // at least one warp for each chunk of heads, at most what the card holds at once
-  const int64_t most = std::max<int64_t>(int64_t(sm_count()) * 4, (sh.chunks + per - 1) / per);
+  const int64_t most = std::max<int64_t>(int64_t(sm_count()) * kCtas, (sh.chunks + per - 1) / per);
   const int64_t grid = std::min((warps + per - 1) / per, most);
-  if (a.interleaved) qk_norm_rope_kernel<kBf16, kLanes, true><<<unsigned(grid), kThreads, 0, s>>>(a, sh, err);
-  else qk_norm_rope_kernel<kBf16, kLanes, false><<<unsigned(grid), kThreads, 0, s>>>(a, sh, err);
+  constexpr int kBytes = kStages * (kThreads / 32) * kPasses * 2 * 32 * 16;
+  const auto kernel = a.interleaved ? qk_norm_rope_kernel<kBf16, kLanes, true, kPasses, kStages>
+                                    : qk_norm_rope_kernel<kBf16, kLanes, false, kPasses, kStages>;
+  if (kBytes > 48 * 1024 &&
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes) != cudaSuccess)
+    return check_launch("qk_norm_rope");
+  kernel<<<unsigned(grid), kThreads, kBytes, s>>>(a, sh, err);
   return check_launch("qk_norm_rope");
+}
+
+template <bool kBf16, int kLanes>
+int launch_size(const KittyQkNormRopeArgs& a, uint32_t* err, cudaStream_t s) {
+  // Stages pay where a resident warp has more than one token (40 heads of 128: 8.0 against
+  // 9.3 us for 1024 tokens, 32 against 40 for 8192, 114 against 119 for 32768) and cost where it
+  // has one (301 tokens of 72 heads: 6.3 and 5.1 us).
+  constexpr int kStaged = 4, kHeads = 32 / kLanes * kStaged;
+  const int64_t chunks = (a.num_q_heads + kHeads - 1) / kHeads + (a.num_k_heads + kHeads - 1) / kHeads;
+  return a.rows * chunks > int64_t(sm_count()) * kCtas * (kThreads / 32) ? launch<kBf16, kLanes, kStaged, 2>(a, err, s)
+                                                                         : launch<kBf16, kLanes, 2, 0>(a, err, s);
 }
 
 template <bool kBf16>
 int launch_dim(const KittyQkNormRopeArgs& a, uint32_t* err, cudaStream_t s) {
-  if (a.head_dim <= 64) return launch<kBf16, 4>(a, err, s);
-  if (a.head_dim <= 128) return launch<kBf16, 8>(a, err, s);
-  return launch<kBf16, 16>(a, err, s);
+  if (a.head_dim <= 64) return launch_size<kBf16, 4>(a, err, s);
+  if (a.head_dim <= 128) return launch_size<kBf16, 8>(a, err, s);
+  return launch_size<kBf16, 16>(a, err, s);
 }
 
 }  // namespace
