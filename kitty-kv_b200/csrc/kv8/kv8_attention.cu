@@ -1,8 +1,11 @@
 // Decode attention over the 8-bit paged cache.
 //
 // Per (slot, KV head, pass of up to 8 kNT query heads) - a segment - with scores in
-// base 2: s_t = sm_scale log2(e) key_scale (q . code_t), and a running maximum m,
-//   l <- l 2^(m - m') + sum_t 2^(s_t - m'),   O <- O 2^(m - m') + value_scale sum_t 2^(s_t - m') code_t.
+// base 2: s_t = sm_scale log2(e) key_scale (q . code_t), and a reference m,
+//   l <- l + sum_t 2^(s_t - m),   O <- O + value_scale sum_t 2^(s_t - m) code_t.
+// The reference is a maximum seen so far, and stays while no score is more than kSlack
+// above it: then the weights need no maximum over the warp and O and l no rescaling, which
+// were a sixth of the instructions and the longest chain of a tile.
 //
 // What bounds it: every cached byte is used by g = Hq / H query heads, 4 g flops a byte
 // (g = 4 ... 16), so it is a read of the cache at HBM speed.  The arithmetic runs on
@@ -21,9 +24,9 @@
 // 8-bit codes become fp16 exactly (e4m3 by conversion, int8 by the exponent trick), so
 // the products are exact and the sums float32.  q is fp16; a bf16 q is scaled by a power
 // of two per head that puts its largest element near the top of fp16's range, which
-// keeps elements down to 2^-29 of it exact.  Weights are rounded to fp16 with 2^14 of
-// headroom; for fp16 outputs, whose own rounding is as small, they are split in two
-// parts (16-bit tails of bf16 slots: two bf16 parts).
+// keeps elements down to 2^-29 of it exact.  Weights are rounded to fp16, off by at most
+// 2^-11 of themselves or 2^-31 of the one at the reference; for fp16 outputs, whose own
+// rounding is as small, they are split in two parts (16-bit tails: two parts of the type).
 //
 // All segments' tiles (kTile tokens of a page, half as many of a tail: about the same
 // bytes) are laid end to end, each segment's behind kSetup units that stand for what a
@@ -39,7 +42,9 @@ namespace kitty8 {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kHead = 14.f;          // weights are kept times 2^kHead, so that small ones stay normal in fp16
+constexpr float kHead = 6.f;           // weights are 2^(score - m + kHead): at most 2^(kHead + kSlack) = 2^14, and
+constexpr float kSlack = 8.f;          // normal in fp16 down to 2^-20 of the one at m
+constexpr float kUnset = -3.402823466e38f;   // no reference yet: any finite score is far above it
 constexpr int kWarps = 4;              // per CTA
 constexpr int kSetup = 2;              // units (tiles) that beginning and ending a segment count as
 constexpr int kAhead = 4;              // tiles that a prefetch asks for
@@ -49,7 +54,7 @@ constexpr int kBatch = 8;              // parts whose loads merge_kernel has in 
 struct Plan {
   int passes, pass_heads;              // query heads of a KV head in passes of pass_heads
   int warps;                           // of the whole grid
-  float* part_ml;                      // [2 warps][pass_heads][2]  maximum, sum
+  float* part_ml;                      // [2 warps][pass_heads][2]  reference, sum
   float* part_o;                       // [2 warps][pass_heads][D]
   int64_t* seg_begin;                  // [segments] first unit of a segment that left parts, -1: stored; then the
                                        // units of a slice
@@ -416,37 +421,58 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
       for (int j = 0; j < 2; ++j) fac[nt][j] = __shfl_sync(0xffffffffu, scale, (2 * lc + j) * 4) * fac16;
     }
 
-    float o[kNT][kOT][4], m[kNT][2], l[kNT][2];
+    float o[kNT][kOT][4], base[kNT][2], l[kNT][2];   // base: the reference less kHead
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
 #pragma unroll
       for (int i = 0; i < kOT; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
-      m[nt][0] = m[nt][1] = -INFINITY;
+      base[nt][0] = base[nt][1] = kUnset;
       l[nt][0] = l[nt][1] = 0.f;
     }
 
-    // Softmax step of one tile: scores s (token rows lr and lr + 8 of each group, two head
-    // columns) become weights 2^(s - m + kHead) and alpha gets the factor of what was
-    // there before.
-    auto softmax = [&](auto& s, int nt, float (&alpha)[2]) {
+    // Weights of one tile: products s (token rows lr and lr + 8 of each group, two head
+    // columns), times f a score, become 2^(score - base).  `there(group, row)`: whether the
+    // token exists.
+    auto weigh = [&](auto& s, int nt, float f0_, float f1_, auto there) {
       constexpr int kGroups = sizeof(s) / sizeof(s[0]);
+      float x[kGroups][4], top = -INFINITY;
+      auto relative = [&]() {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float top = m[nt][j];
+        for (int k = 0; k < kGroups; ++k)
 #pragma unroll
-        for (int k = 0; k < kGroups; ++k) top = fmaxf(top, fmaxf(s[k][j], s[k][2 + j]));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-        const float ref = top == -INFINITY ? 0.f : top;      // nothing yet: all weights 0
-        alpha[j] = ex2(m[nt][j] - ref);
-        m[nt][j] = top;
+          for (int i = 0; i < 4; ++i) {
+            x[k][i] = there(k, i / 2) ? fmaf(s[k][i], i & 1 ? f1_ : f0_, -base[nt][i & 1]) : -INFINITY;
+            top = fmaxf(top, x[k][i]);
+          }
+      };
+      relative();
+      if (!__all_sync(0xffffffffu, top <= kHead + kSlack)) {   // a score far above the reference (or none yet, or NaN)
 #pragma unroll
-        for (int k = 0; k < kGroups; ++k) {
-          s[k][j] = ex2(s[k][j] - (ref - kHead));
-          s[k][2 + j] = ex2(s[k][2 + j] - (ref - kHead));
+        for (int j = 0; j < 2; ++j) {
+          float best = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < kGroups; ++k) {
+            if (there(k, 0)) best = fmaxf(best, s[k][j] * (j ? f1_ : f0_));
+            if (there(k, 1)) best = fmaxf(best, s[k][2 + j] * (j ? f1_ : f0_));
+          }
+          best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 4));
+          best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 8));
+          best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 16));
+          const float now = fmaxf(base[nt][j], best - kHead), alpha = ex2(base[nt][j] - now);
+          base[nt][j] = now;
+          l[nt][j] *= alpha;
+#pragma unroll
+          for (int i = 0; i < kOT; ++i) {
+            o[nt][i][j] *= alpha;
+            o[nt][i][2 + j] *= alpha;
+          }
         }
+        relative();
       }
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[k][i] = ex2(x[k][i]);
     };
 
     for (int t = t0; t < p1; ++t) {
@@ -486,34 +512,23 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
         load_tail_keys(t + 1);
       }
       uint32_t wb[kNT][kMT][kParts][2];           // weights as the other operand: tokens 0..7 and 8..15 of a group
-      float alpha[kNT][2];
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) {
-#pragma unroll
-        for (int mt = 0; mt < kMT; ++mt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[nt][mt][i] = ok_now ? s[nt][mt][i] * (fac[nt][i & 1] * ks_now) : -INFINITY;
-        softmax(s[nt], nt, alpha[nt]);
-        float sum[2] = {0.f, 0.f};
+        weigh(s[nt], nt, fac[nt][0] * ks_now, fac[nt][1] * ks_now, [&](int, int) { return ok_now; });
 #pragma unroll
         for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const uint32_t hi = dev::from_f2<false>(s[nt][mt][2 * r], s[nt][mt][2 * r + 1]);
-            const float2 back = dev::to_f2<false>(hi);
             wb[nt][mt][0][r] = transpose8x8(hi);
             if constexpr (kParts == 2) {
+              const float2 back = dev::to_f2<false>(hi);
               wb[nt][mt][kParts - 1][r] =
                   transpose8x8(dev::from_f2<false>(s[nt][mt][2 * r] - back.x, s[nt][mt][2 * r + 1] - back.y));
-              sum[0] += s[nt][mt][2 * r];
-              sum[1] += s[nt][mt][2 * r + 1];
-            } else {                              // the sum of what the product uses
-              sum[0] += back.x;
-              sum[1] += back.y;
             }
+            l[nt][0] += s[nt][mt][2 * r];
+            l[nt][1] += s[nt][mt][2 * r + 1];
           }
-        l[nt][0] = l[nt][0] * alpha[nt][0] + sum[0];
-        l[nt][1] = l[nt][1] * alpha[nt][1] + sum[1];
       }
       const float vmul = ok_now ? vs_now : 0.f;
 #pragma unroll
@@ -542,7 +557,7 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
 #pragma unroll
             for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) o[nt][i][e] = fmaf(acc[nt][e], vmul, o[nt][i][e] * alpha[nt][e & 1]);
+              for (int e = 0; e < 4; ++e) o[nt][i][e] = fmaf(acc[nt][e], vmul, o[nt][i][e]);
           }
       if (t + 1 < p1) load_values();
       else if (t + 1 < t1) load_tail_values(t + 1);
@@ -573,13 +588,9 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
         }
       if (t + 1 < t1) load_tail_keys(t + 1);
       uint32_t wb[kNT][2][2];                     // two parts of the tails' type
-      float alpha[kNT][2];
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          s[nt][0][i] = i / 2 < kTailRows && tok + 8 * (i / 2) < tl.tail ? s[nt][0][i] * fac16 : -INFINITY;
-        softmax(s[nt], nt, alpha[nt]);
+        weigh(s[nt], nt, fac16, fac16, [&](int, int row) { return row < kTailRows && tok + 8 * row < tl.tail; });
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const uint32_t hi = dev::from_f2<kBf16>(s[nt][0][2 * r], s[nt][0][2 * r + 1]);
@@ -587,8 +598,8 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
           wb[nt][0][r] = transpose8x8(hi);
           wb[nt][1][r] = transpose8x8(dev::from_f2<kBf16>(s[nt][0][2 * r] - back.x, s[nt][0][2 * r + 1] - back.y));
         }
-        l[nt][0] = l[nt][0] * alpha[nt][0] + (s[nt][0][0] + s[nt][0][2]);
-        l[nt][1] = l[nt][1] * alpha[nt][1] + (s[nt][0][1] + s[nt][0][3]);
+        l[nt][0] += s[nt][0][0] + s[nt][0][2];
+        l[nt][1] += s[nt][0][1] + s[nt][0][3];
       }
 #pragma unroll
       for (int vh = 0; vh < kVH; ++vh)
@@ -602,8 +613,6 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
           const uint32_t a2 = prmt(w2, w3, 0x5410), a3 = prmt(w2, w3, 0x7632);
 #pragma unroll
           for (int nt = 0; nt < kNT; ++nt) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[nt][i][e] *= alpha[nt][e & 1];
             mma<kBf16>(o[nt][i], a0, a1, a2, a3, wb[nt][0][0], wb[nt][0][1]);
             mma<kBf16>(o[nt][i], a0, a1, a2, a3, wb[nt][1][0], wb[nt][1][1]);
           }
@@ -634,7 +643,7 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
         if (lr == 0) {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            s_m[w][nt * 8 + 2 * lc + j] = m[nt][j];
+            s_m[w][nt * 8 + 2 * lc + j] = base[nt][j];
             s_l[w][nt * 8 + 2 * lc + j] = l[nt][j];
           }
         }
@@ -652,12 +661,11 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
           float top = s_m[0][col];
 #pragma unroll
           for (int i = 1; i < kWarps; ++i) top = fmaxf(top, s_m[i][col]);
-          const float ref = top == -INFINITY ? 0.f : top;
-          m[nt][j] = top;
+          base[nt][j] = top;
           l[nt][j] = 0.f;
 #pragma unroll
           for (int i = 0; i < kWarps; ++i) {
-            k[i][j] = ex2(s_m[i][col] - ref);
+            k[i][j] = ex2(s_m[i][col] - top);
             l[nt][j] = fmaf(k[i][j], s_l[i][col], l[nt][j]);
           }
         }
@@ -690,7 +698,7 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
         float* part = plan.part_o + (place * plan.pass_heads + qh) * D;
         if (!all_here && lr == 0 && x0 == 0) {
           float* ml = plan.part_ml + (place * plan.pass_heads + qh) * 2;
-          ml[0] = m[nt][j];
+          ml[0] = base[nt][j];
           ml[1] = l[nt][j];
         }
 #pragma unroll
@@ -712,7 +720,7 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
 // Joins the parts of a segment's query head: out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M)
 // l_i; zeros for an empty slot.  Where segments are few, each has many parts: the team is
 // a CTA, whose threads form groups of one thread for each 16-byte vector of the head; the
-// groups take the parts in turn, each with its own maximum, and are joined in order.  Where
+// groups take the parts in turn, each with its own reference, and are joined in order.  Where
 // they are many, most were stored by their warp and the others have a few parts: the team is
 // a warp.
 template <int kTile, bool kBf16, int kTeam>
