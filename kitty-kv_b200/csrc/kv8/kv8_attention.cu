@@ -51,13 +51,18 @@ constexpr int kAhead = 4;              // tiles that a prefetch asks for
 constexpr int kMergeThreads = 256;
 constexpr int kBatch = 8;              // parts whose loads merge_kernel has in flight
 
+// What attention_kernel leaves about a segment for merge_kernel.
+struct alignas(16) Note {
+  int64_t begin;                       // its first unit, where it left parts
+  int64_t units;                       // its units; 0: an empty slot; -1: stored already
+};
+
 struct Plan {
   int passes, pass_heads;              // query heads of a KV head in passes of pass_heads
   int warps;                           // of the whole grid
   float* part_ml;                      // [2 warps][pass_heads][2]  reference, sum
   float* part_o;                       // [2 warps][pass_heads][D]
-  int64_t* seg_begin;                  // [segments] first unit of a segment that left parts, -1: stored; then the
-                                       // units of a slice
+  Note* notes;                         // [segments + 1], the last holding the units of a slice
 };
 
 __device__ __forceinline__ uint4 ld_stream(const void* p) {
@@ -113,6 +118,10 @@ __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t
   }
 }
 
+// Tokens of a tile of a page.
+template <int kDim>
+constexpr int kTileOf = kDim == 256 ? 16 : 32;
+
 // Tiles of a slot's segments: its whole pages, then its tail.
 struct Tiles {
   int paged, all, tail;                // tiles in pages, all tiles, tail tokens
@@ -143,41 +152,102 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
   return ((a | b) >> 32) == 0 ? int64_t(uint32_t(a) / uint32_t(b)) : a / b;
 }
 
-// The units of the whole batch, and where batch row `b` or unit `f` lies among them.  Row
-// b has `per_row` = H * passes segments of equal length.  By the whole warp.
-struct Place {
-  int64_t total;       // units of all rows
-  int64_t begin;       // first unit of the segment found
-  int b, seg;          // its batch row and its index among the row's segments
-};
+// Row b has `per_row` = H * passes segments of equal length.
 template <int kTile>
 __device__ __forceinline__ int units_of_row(const KittyKv8AttentionArgs& a, int b, uint32_t* err = nullptr) {
   return b < a.batch ? tiles_of<kTile>(a.cache, tokens_of(a, b, err)).units() : 0;
 }
+
+// The rows before a place, in units: thread t of a CTA has rows [t rows_each, (t + 1)
+// rows_each) (one warp at a time took 9 us for 256 rows, the CTA together takes 1).
+struct Rows {
+  int64_t before[kWarps * 32];         // units of the rows before each thread's
+  int64_t total[kWarps];
+};
+
+// By the whole CTA: fills `s`; returns the units of all rows.  The first CTA also flags rows
+// whose slot or length is out of range, and notes empty ones.
 template <int kTile>
-__device__ __forceinline__ int64_t total_units(const KittyKv8AttentionArgs& a, int first, int per_row) {
-  const int lane = threadIdx.x & 31;
-  int64_t sum = first;
+__device__ __forceinline__ int64_t scan_rows(const KittyKv8AttentionArgs& a, const Plan& plan, int per_row,
+                                             int rows_each, Rows& s, uint32_t* err) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  int64_t mine = 0;
 #pragma unroll 4
-  for (int b = lane + 32; b < a.batch; b += 32) sum += units_of_row<kTile>(a, b);
+  for (int i = 0; i < rows_each; ++i) {
+    const int b = tid * rows_each + i, n = units_of_row<kTile>(a, b, blockIdx.x == 0 ? err : nullptr);
+    mine += n;
+    if (blockIdx.x == 0 && n == 0 && b < a.batch)
+      for (int k = 0; k < per_row; ++k) plan.notes[int64_t(b) * per_row + k].units = 0;
+  }
+  int64_t incl = mine;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  return sum * per_row;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) s.total[tid >> 5] = incl;
+  __syncthreads();
+  int64_t before = incl - mine, all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < tid >> 5) before += s.total[w];
+    all += s.total[w];
+  }
+  s.before[tid] = before;
+  __syncthreads();
+  return all;
 }
-// The segment that holds unit f (f < total); `first`: the units of row `lane`.
+
+struct Place {
+  int64_t begin;       // first unit of the segment found
+  int b, seg;          // its batch row and its index among the row's segments
+};
+// By the whole warp, for at most 32 rows: `incl` gets the units up to and with row `lane`'s;
+// returns those of all rows.  (No barrier, and no second look at the lengths.)
 template <int kTile>
-__device__ __forceinline__ Place locate(const KittyKv8AttentionArgs& a, int first, int per_row, int64_t f) {
+__device__ __forceinline__ int64_t scan_few(const KittyKv8AttentionArgs& a, const Plan& plan, int per_row, int64_t& one,
+                                            int64_t& incl, uint32_t* err) {
   const int lane = threadIdx.x & 31;
-  Place r{0, 0, 0, 0};
-  int64_t before = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 32) {
-    const int one = b0 == 0 ? first : units_of_row<kTile>(a, b0 + lane);
+  const bool flags = blockIdx.x == 0 && threadIdx.x < 32;
+  one = units_of_row<kTile>(a, lane, flags ? err : nullptr);
+  if (flags && one == 0 && lane < a.batch)
+    for (int k = 0; k < per_row; ++k) plan.notes[int64_t(lane) * per_row + k].units = 0;
+  incl = one;
+  for (int o = 1; o < a.batch; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  return __shfl_sync(0xffffffffu, incl, a.batch - 1);
+}
+__device__ __forceinline__ Place locate_few(int per_row, int64_t one, int64_t incl, int64_t f) {
+  const int64_t start = (incl - one) * per_row;
+  const int b = __ffs(__ballot_sync(0xffffffffu, f >= start && f < incl * per_row)) - 1;
+  const int64_t at = __shfl_sync(0xffffffffu, start, b), len = __shfl_sync(0xffffffffu, one, b);
+  const int seg = int(quotient(f - at, len));
+  return Place{at + seg * len, b, seg};
+}
+
+// By the whole warp: the segment that holds unit f (less than there are).
+template <int kTile>
+__device__ __forceinline__ Place locate(const KittyKv8AttentionArgs& a, int per_row, int rows_each, const Rows& s,
+                                        int64_t f) {
+  const int lane = threadIdx.x & 31;
+  int found = 0;                       // threads whose rows begin at or before f
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) found += __popc(__ballot_sync(0xffffffffu, s.before[w * 32 + lane] * per_row <= f));
+  const int b0 = (found - 1) * rows_each;
+  Place r{0, b0, 0};
+  int64_t before = s.before[found - 1] * per_row;
+  for (int i = 0; i < rows_each; i += 32) {
+    const int one = i + lane < rows_each ? units_of_row<kTile>(a, b0 + i + lane) : 0;
     int64_t incl = int64_t(one) * per_row;
     const int64_t mine = incl;
+    if (rows_each > 1) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
     }
     const int64_t start = before + incl - mine;
     const uint32_t hit = __ballot_sync(0xffffffffu, f >= start && f < start + mine);
@@ -185,7 +255,7 @@ __device__ __forceinline__ Place locate(const KittyKv8AttentionArgs& a, int firs
       const int src = __ffs(hit) - 1;
       const int64_t at = __shfl_sync(0xffffffffu, start, src);
       const int len = __shfl_sync(0xffffffffu, one, src);
-      r.b = b0 + src;
+      r.b = b0 + i + src;
       r.seg = int(quotient(f - at, len));
       r.begin = at + int64_t(r.seg) * len;
       return r;
@@ -211,7 +281,7 @@ constexpr int kMinCtas = kDim == 64 ? 4 : kDim == 128 ? 3 : 1;
 template <int kDim, int kNT, bool kWhole, bool kBf16, int kCode>
 __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
     attention_kernel(KittyKv8AttentionArgs a, Plan plan, uint32_t* err) {
-  constexpr int kTile = kDim == 256 ? 16 : 32;      // tokens of a page tile
+  constexpr int kTile = kTileOf<kDim>;              // tokens of a page tile
   constexpr int kTailTile = kTile / 2;              // tokens of a tail tile
   constexpr int kMT = kTile / 16;                   // 16-token groups of a page tile
   constexpr int kKC = kDim / 64;                    // 64-channel column blocks of a key row
@@ -232,15 +302,17 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
   const float fac16 = a.sm_scale * kLog2e;
 
   // this warp's slice [f, f_end)
-  const int first = units_of_row<kTile>(a, lane, warp == 0 ? err : nullptr);
-  if (warp == 0)
-    for (int b = lane + 32; b < a.batch; b += 32) tokens_of(a, b, err);
-  const int64_t total = total_units<kTile>(a, first, per_row);
+  __shared__ Rows s_rows;
+  const int rows_each = (a.batch + kWarps * 32 - 1) / (kWarps * 32);
+  int64_t row_one = 0, row_incl = 0;
+  const bool few = a.batch <= 32;
+  const int64_t total = (few ? scan_few<kTile>(a, plan, per_row, row_one, row_incl, err)
+                             : scan_rows<kTile>(a, plan, per_row, rows_each, s_rows, err)) * per_row;
   const int64_t per_warp = quotient(total + plan.warps - 1, plan.warps);
   const int64_t f0 = warp * per_warp, f_end = min(total, f0 + per_warp);
   if (f0 >= f_end) return;
-  if (warp == 0 && lane == 0) plan.seg_begin[int64_t(a.batch) * per_row] = per_warp;
-  const Place at = locate<kTile>(a, first, per_row, f0);
+  if (warp == 0 && lane == 0) plan.notes[int64_t(a.batch) * per_row].units = per_warp;
+  const Place at = few ? locate_few(per_row, row_one, row_incl, f0) : locate<kTile>(a, per_row, rows_each, s_rows, f0);
   int b = at.b, seg = at.seg;
   int64_t begin = at.begin;
 
@@ -630,7 +702,7 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
         l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 16);
       }
     const bool all_here = t0 == 0 && t1 == tl.all;
-    if (t0 == 0 && lane == 0) plan.seg_begin[segment] = all_here ? -1 : here;
+    if (t0 == 0 && lane == 0) plan.notes[segment] = all_here ? Note{0, -1} : Note{here, end - here};
     const bool together = cta_inside(blockIdx.x, per_warp, here, end);
     int x0 = 0, x1 = kOT / 2;                       // pairs of output tiles that this warp stores
     const int w = threadIdx.x >> 5;
@@ -717,29 +789,27 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
   }
 }
 
-// Joins the parts of a segment's query head: out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M)
-// l_i; zeros for an empty slot.  Where segments are few, each has many parts: the team is
-// a CTA, whose threads form groups of one thread for each 16-byte vector of the head; the
-// groups take the parts in turn, each with its own reference, and are joined in order.  Where
-// they are many, most were stored by their warp and the others have a few parts: the team is
-// a warp.
+// Joins the parts of a segment: out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i; zeros for an
+// empty slot.  Where segments are few, each has many parts: the team is a CTA for one query
+// head, whose threads form groups of one thread for each 16-byte vector of the head; the
+// groups take the parts in turn, each with its own reference, and are joined in order.
+// Otherwise the team is a warp, for `heads_each` heads.
 template <int kTile, bool kBf16, int kTeam>
-__global__ void __launch_bounds__(kMergeThreads) merge_kernel(KittyKv8AttentionArgs a, Plan plan) {
+__global__ void __launch_bounds__(kMergeThreads) merge_kernel(KittyKv8AttentionArgs a, Plan plan, int heads_each) {
   __shared__ float4 s_sum[kTeam == 32 ? 1 : kTeam];
   __shared__ float s_l[kTeam == 32 ? 1 : kTeam], s_m[kTeam == 32 ? 1 : kTeam];
   const KittyKv8Cache& c = a.cache;
   const int tid = threadIdx.x % kTeam;
   const int D = c.head_dim, g = a.num_q_heads / c.num_heads, per_row = c.num_heads * plan.passes;
   const uint32_t team = blockIdx.x * (kMergeThreads / kTeam) + threadIdx.x / kTeam;
-  const uint32_t segment = team / plan.pass_heads;
-  const int head = int(team - segment * plan.pass_heads);
+  const uint32_t per_segment = (plan.pass_heads + heads_each - 1) / heads_each, segment = team / per_segment;
   const int b = int(segment / per_row), seg = int(segment - uint32_t(b) * per_row);
   const int h = seg / plan.passes, q0 = (seg - h * plan.passes) * plan.pass_heads;
-  const int units = units_of_row<kTile>(a, b);
-  // Where the segment begins: a few rows are looked through while attention_kernel still
-  // runs, of many the kernel has left a note.
-  int64_t begin = -1, per_warp = 1;
-  if constexpr (kTeam != 32) {
+  const int first = int(team - segment * per_segment) * heads_each;
+  const int heads = min(min(plan.pass_heads, g - q0) - first, heads_each);
+  Note note{0, -2};
+  int64_t per_warp = 1;
+  if (kTeam != 32 && a.batch <= 64) {                  // where the segment begins, while attention_kernel still runs
     int64_t before = 0, total = 0;
     for (int i = threadIdx.x & 31; i < a.batch; i += 32) {
       const int64_t n = units_of_row<kTile>(a, i);
@@ -752,22 +822,24 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(KittyKv8AttentionA
       before += __shfl_xor_sync(0xffffffffu, before, o);
     }
     per_warp = max(quotient(total * per_row + plan.warps - 1, plan.warps), int64_t(1));
-    begin = before * per_row + int64_t(seg) * units;
+    note.units = units_of_row<kTile>(a, b);
+    note.begin = before * per_row + int64_t(seg) * note.units;
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");   // attention_kernel is done and its parts are visible
-  if (b >= a.batch || q0 + head >= g) return;
-  uint16_t* out = static_cast<uint16_t*>(a.out) + b * a.out_s_seq + int64_t(h * g + q0 + head) * a.out_s_head;
-  const int vecs = D / 4;                              // (at most 64)
-  if (units == 0) {
-    for (int v = tid; v < vecs; v += kTeam) *reinterpret_cast<uint2*>(out + v * 4) = make_uint2(0, 0);
+  if (b >= a.batch || heads <= 0) return;
+  if (note.units == -2) {
+    note = plan.notes[segment];
+    per_warp = plan.notes[int64_t(a.batch) * per_row].units;
+  }
+  if (note.units < 0) return;                          // stored by its warp
+  uint16_t* out = static_cast<uint16_t*>(a.out) + b * a.out_s_seq + int64_t(h * g + q0 + first) * a.out_s_head;
+  const int vecs = D / 4, work = heads * vecs;         // (vecs at most 64)
+  if (note.units == 0) {
+    for (int u = tid; u < work; u += kTeam)
+      *reinterpret_cast<uint2*>(out + (u / vecs) * a.out_s_head + (u % vecs) * 4) = make_uint2(0, 0);
     return;
   }
-  if constexpr (kTeam == 32) {
-    begin = plan.seg_begin[segment];
-    per_warp = plan.seg_begin[int64_t(a.batch) * per_row];
-    if (begin < 0) return;
-  }
-  const int64_t end = begin + units, per_cta = per_warp * kWarps;
+  const int64_t begin = note.begin, end = begin + note.units, per_cta = per_warp * kWarps;
   const int w0 = int(quotient(begin + kSetup, per_warp)), w1 = int(quotient(end - 1, per_warp));
   if (w0 == w1) return;                                // stored by its warp
   // its parts: warps w0 .., whole CTAs c0 .. c1 - 1, warps .. w1
@@ -777,12 +849,13 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(KittyKv8AttentionA
   const int parts = n2 ? n1 + n2 + (w1 - c1 * kWarps + 1) : n1;
   auto place = [&](int i) {
     const int w = i < n1 ? w0 + i : i < n1 + n2 ? (c0 + i - n1) * kWarps : c1 * kWarps + (i - n1 - n2);
-    return (2 * int64_t(w) + (begin > w * per_warp)) * plan.pass_heads + head;
+    return (2 * int64_t(w) + (begin > w * per_warp)) * plan.pass_heads + first;
   };
   const int groups = kTeam == 32 ? 1 : kTeam / vecs;
-  for (int v0 = 0; v0 < vecs; v0 += kTeam) {           // (a second round: a warp and more than 128 channels)
-    const int group = kTeam == 32 ? 0 : tid / vecs, v = kTeam == 32 ? v0 + tid : tid - group * vecs;
-    const bool mine = v < vecs && group < groups;
+  for (int u0 = 0; u0 < work; u0 += kTeam) {           // (a CTA: one round)
+    const int group = kTeam == 32 ? 0 : tid / vecs, u = kTeam == 32 ? u0 + tid : tid - group * vecs;
+    const int head = kTeam == 32 ? u / vecs : 0, v = u - head * vecs;
+    const bool mine = u < work && group < groups;
     float top = -INFINITY, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int i0 = group; mine && i0 < parts; i0 += groups * kBatch) {
@@ -794,7 +867,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(KittyKv8AttentionA
         ml[k] = make_float2(-INFINITY, 0.f);
         p[k] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (i < parts) {
-          const int64_t at = place(i);
+          const int64_t at = place(i) + head;
           ml[k] = *reinterpret_cast<const float2*>(plan.part_ml + at * 2);
           p[k] = *reinterpret_cast<const float4*>(plan.part_o + at * D + v * 4);
         }
@@ -838,7 +911,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(KittyKv8AttentionA
     }
     if (mine && group == 0) {
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      *reinterpret_cast<uint2*>(out + v * 4) =
+      *reinterpret_cast<uint2*>(out + head * a.out_s_head + v * 4) =
           make_uint2(dev::from_f2<kBf16>(acc.x * inv, acc.y * inv), dev::from_f2<kBf16>(acc.z * inv, acc.w * inv));
     }
   }
@@ -847,17 +920,18 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(KittyKv8AttentionA
 // merge_kernel behind attention_kernel, as its programmatic dependent: it is launched while
 // the other runs and waits in front of the first part that it reads.
 template <int kTile, bool kBf16, int kTeam>
-cudaError_t launch_merge(const KittyKv8AttentionArgs& a, const Plan& plan, dim3 grid, cudaStream_t s) {
+cudaError_t launch_merge(const KittyKv8AttentionArgs& a, const Plan& plan, int heads_each, cudaStream_t s) {
+  const unsigned teams = unsigned(a.batch) * a.cache.num_heads * plan.passes * ((plan.pass_heads + heads_each - 1) / heads_each);
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
+  cfg.gridDim = dim3((teams + kMergeThreads / kTeam - 1) / (kMergeThreads / kTeam));
   cfg.blockDim = kMergeThreads;
   cfg.stream = s;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, merge_kernel<kTile, kBf16, kTeam>, a, plan);
+  return cudaLaunchKernelEx(&cfg, merge_kernel<kTile, kBf16, kTeam>, a, plan, heads_each);
 }
 
 // Resident CTAs per SM that a kernel's registers allow (asked once per kernel).
@@ -876,14 +950,14 @@ int resident() {
   return known;
 }
 
-// The workspace: the segments' begins and the slice's units, the parts' maxima and sums, and
+// The workspace: the segments' notes, the parts' references and sums, and
 // their outputs, each from a 256-byte boundary.  Returns its bytes.
 size_t lay_out(Plan& plan, const KittyKv8AttentionArgs& a, uint8_t* base) {
   const auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   const size_t segments = size_t(a.batch) * a.cache.num_heads * plan.passes;
   const size_t parts = size_t(2) * plan.warps * plan.pass_heads;
-  const size_t begins = up((segments + 1) * 8), ml = up(parts * 8);
-  plan.seg_begin = reinterpret_cast<int64_t*>(base);
+  const size_t begins = up((segments + 1) * sizeof(Note)), ml = up(parts * 8);
+  plan.notes = reinterpret_cast<Note*>(base);
   plan.part_ml = reinterpret_cast<float*>(base + begins);
   plan.part_o = reinterpret_cast<float*>(base + begins + ml);
   return begins + ml + parts * a.cache.head_dim * 4;
@@ -900,13 +974,14 @@ int launch(const KittyKv8AttentionArgs& a, Plan plan, uint32_t* err, cudaStream_
   attention_kernel<kDim, kNT, kWhole, kBf16, kCode><<<grid, kWarps * 32, 0, s>>>(a, plan, err);
   const int rc = check_launch("kv8_attention");
   if (rc != KITTY_OK) return rc;
-  constexpr int kTile = kDim == 256 ? 16 : 32;
-  // Few segments are shared by many warps each, many segments are mostly one warp's own.
-  const unsigned segments = unsigned(a.batch) * a.cache.num_heads * plan.passes, teams = segments * plan.pass_heads;
-  const unsigned per = kMergeThreads / 32;
-  const cudaError_t e = segments < unsigned(plan.warps) / 4
-                            ? launch_merge<kTile, kBf16, kMergeThreads>(a, plan, dim3(teams), s)
-                            : launch_merge<kTile, kBf16, 32>(a, plan, dim3((teams + per - 1) / per), s);
+  // Many warps to a segment: a CTA joins a head.  Otherwise a warp joins as many heads as it has
+  // lanes for: of 256 mixed lengths, 2048 segments of 5 heads, in 58.5 us all told (one head a
+  // warp 60.5, all five 60.8).
+  const int64_t segments = int64_t(a.batch) * a.cache.num_heads * plan.passes;
+  const int heads_each = std::min(std::max(1, 128 / a.cache.head_dim), plan.pass_heads);
+  const cudaError_t e = segments * 32 < plan.warps
+                            ? launch_merge<kTileOf<kDim>, kBf16, kMergeThreads>(a, plan, 1, s)
+                            : launch_merge<kTileOf<kDim>, kBf16, 32>(a, plan, heads_each, s);
   return e == cudaSuccess ? KITTY_OK : fail(KITTY_ERR_CUDA, "kv8_attention (merge)", cudaGetErrorString(e));
 }
 
