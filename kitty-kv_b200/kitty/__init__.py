@@ -11,6 +11,7 @@ from .layout import PageCentricKVLayoutManager
 from .pipeline import KittyInferencePipeline
 from .attention import KittyPagedAttention, KittyAttentionFactory
 from .batched import BatchedKVCache
+from .paged8 import PagedKVCache8
 
 __version__ = "0.1.0+b200"
 __description__ = ("2-bit KV Cache Quantization with per-channel boosted precision and Dense-Sparse "
@@ -24,4 +25,5 @@ __all__ = [
     "KittyPagedAttention",
     "KittyAttentionFactory",
     "BatchedKVCache",
+    "PagedKVCache8",
 ]

@@ -172,3 +172,14 @@ def test_rope_table_is_exact_far_out():
                 dict(inv_freq=torch.ones(5))):
         with pytest.raises(RuntimeError):
             K.rope_table(**{**dict(max_positions=4, rotary_dim=64), **bad})
+
+
+def test_cache_class_is_refused_on_the_cpu_and_for_bad_shapes():
+    import kitty
+    ok = dict(num_layers=1, num_kv_heads=2, head_dim=64, max_seq_len=128, device="cpu")
+    with pytest.raises(RuntimeError, match="CUDA"):
+        kitty.PagedKVCache8(kitty.KittyConfig(**ok), 2)
+    for cfg, kw in ((dict(head_dim=72), {}), (dict(head_dim=288), {}), ({}, dict(page_size=48)), ({}, dict(page_size=0)),
+                    ({}, dict(page_size=512)), ({}, dict(codes="int4"))):
+        with pytest.raises(RuntimeError):
+            kitty.PagedKVCache8(kitty.KittyConfig(**{**ok, **cfg, "device": "cuda:0"}), 2, **kw)
