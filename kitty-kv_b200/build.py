@@ -88,7 +88,7 @@ def _torch_module(module: Path, src: Path, lib: Path, verbose: bool) -> None:
            *(f"-isystem{d}" for d in (root / "include", root / "include" / "torch" / "csrc" / "api" / "include",
                                       cuda / "include", sysconfig.get_paths()["include"])),
            str(src), "-o", str(tmp), str(lib), "-Wl,-rpath,$ORIGIN/..", f"-L{root / 'lib'}",
-           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ltorch_cuda"]
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)

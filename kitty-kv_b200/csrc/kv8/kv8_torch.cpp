@@ -8,6 +8,8 @@
 
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -75,6 +77,11 @@ bool row_strides(const Tensor& t, int64_t& s0, int64_t& s1) {
          reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }
 
+// A contiguous tensor on the device of `like` (without the way through the dispatcher).
+Tensor make(at::IntArrayRef shape, const Tensor& like) {
+  return at::detail::empty_cuda(shape, like.scalar_type(), like.device(), std::nullopt);
+}
+
 // An input of aligned rows, copied if it has none.
 const void* input_rows(Tensor& t, int64_t& s0, int64_t& s1) {
   if (!row_strides(t, s0, s1)) {
@@ -88,7 +95,7 @@ const void* input_rows(Tensor& t, int64_t& s0, int64_t& s1) {
 // A caller's output: refused if its rows are not aligned or overlap.  Undefined: made here.
 void* output_rows(Tensor& t, const Tensor& like, const char* name, int64_t& s0, int64_t& s1) {
   if (!t.defined()) {
-    t = at::empty(like.sizes(), like.options());
+    t = make(like.sizes(), like);
     s0 = like.size(1) * like.size(2);
     s1 = like.size(2);
     return t.data_ptr();
@@ -282,7 +289,7 @@ PyObject* read(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
   a.seq_map = index(map, "seq_map", n);
   const int64_t shape[3] = {rows, a.cache.num_heads, a.cache.head_dim};
   for (Tensor& t : out) {
-    if (!t.defined()) t = at::empty(shape, c.tail_k.options());
+    if (!t.defined()) t = make(shape, c.tail_k);
     TORCH_CHECK(t.sizes() == at::IntArrayRef(shape) && t.scalar_type() == c.tail_k.scalar_type() && t.is_contiguous(),
                 "key_out and value_out must be (", rows, ", ", shape[1], ", ", shape[2], ") ", c.tail_k.scalar_type(),
                 ", contiguous");
@@ -324,8 +331,9 @@ PyObject* attention(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
   a.num_q_heads = i32(hq, "Hq");
   const c10::cuda::CUDAGuard guard(call.device);
   check(kitty_kv8_attention_workspace_size(&a, &a.workspace_bytes), "kitty_kv8_attention_workspace_size");
-  const Tensor scratch = at::empty({int64_t(a.workspace_bytes)}, q.options().dtype(at::kByte));
-  a.workspace = scratch.data_ptr();
+  // from the allocator of this stream (and of this graph, in a capture), and back to it on return
+  const c10::DataPtr scratch = c10::cuda::CUDACachingAllocator::get()->allocate(a.workspace_bytes);
+  a.workspace = scratch.get();
   launch(call, kitty_kv8_attention, a, "kitty_kv8_attention");
   return THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
