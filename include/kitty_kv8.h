@@ -29,7 +29,7 @@
  * of bounds, and set a sticky bit (kitty_kv8_error_flags):
  *   bit 1  a page number outside the pool, or a block past the block table's row
  *   bit 2  row offsets that decrease, are negative or pass the rows of the call
- *   bit 3  a slot outside the cache, or a slot repeated in one write
+ *   bit 3  a slot past the cache, or a slot repeated in one write
  *   bit 4  a negative length, a length past the block table's row, or tokens read past it
  *   bit 5  a position past the rotary table
  */
@@ -87,7 +87,7 @@ typedef struct KittyKv8Cache {
  * key / value (row r, head h, channel c at base + r*s_row + h*s_head + c; 16-byte
  * aligned rows) behind the lengths[slot] tokens that it has, slot = seq_map[i] (NULL:
  * i).  row_offsets NULL: one row each, n == rows.  Rows behind the last offset are
- * ignored.  Blocks that fill are quantised into their pages, which block_table must
+ * ignored, and so are entries of a negative slot (padding).  Blocks that fill are quantised into their pages, which block_table must
  * hold; the rest goes to the tail.  `lengths` is not changed: the caller adds the new
  * tokens before it reads the cache.  One launch.  A slot given twice keeps its first
  * entry. */
@@ -106,7 +106,8 @@ int kitty_kv8_write(const KittyKv8WriteArgs* args, void* stream);
 /* Read tokens back to 16 bits: entry i's rows row_offsets[i] .. row_offsets[i+1] - 1 of
  * key / value ([rows][H][D], contiguous, 16-byte aligned) receive tokens first[i] ..
  * (NULL: from 0) of slot seq_map[i] (NULL: i).  Rows behind the last offset, and rows
- * whose token the slot does not have, are left as they were.  One launch. */
+ * whose token the slot does not have, are left as they were, as are those of a negative
+ * slot (padding).  One launch. */
 typedef struct KittyKv8ReadArgs {
   KittyKv8Cache cache;
   void* key;
@@ -121,7 +122,7 @@ int kitty_kv8_read(const KittyKv8ReadArgs* args, void* stream);
 
 /* Decode attention: out[b][qh] = softmax(sm_scale * q[b][qh] . k) . v over the
  * lengths[slot] tokens of slot seq_map[b] (NULL: b), KV head qh / (Hq / H); zeros for
- * an empty slot.  q and out have the cache's 16-bit type; sums and softmax statistics
+ * an empty slot and for a negative one (padding).  q and out have the cache's 16-bit type; sums and softmax statistics
  * are float32.  The workspace (16-byte aligned) holds the partial results of
  * sequences that several warps share; calls that overlap must not share one. */
 typedef struct KittyKv8AttentionArgs {

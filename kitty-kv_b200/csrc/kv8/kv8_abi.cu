@@ -21,7 +21,7 @@ int check_launch(const char* what) {
 }
 
 int sm_count() {
-  static int known[kMaxDevices];     // 0: not asked yet (a benign race writes the same value)
+  static std::atomic<int> known[kMaxDevices];     // 0: not asked yet
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); return 148; }
   if (dev < kMaxDevices && known[dev]) return known[dev];
@@ -34,11 +34,11 @@ int sm_count() {
 }
 
 uint32_t* error_word() {
-  static void* known[kMaxDevices];   // the symbol's address on each device, fixed for the process
+  static std::atomic<void*> known[kMaxDevices];   // the symbol's address on each device, fixed for the process
   int dev = 0;
   void* p = nullptr;
   if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); return nullptr; }
-  if (dev < kMaxDevices && known[dev]) return static_cast<uint32_t*>(known[dev]);
+  if (dev < kMaxDevices && known[dev]) return static_cast<uint32_t*>(known[dev].load());
   if (cudaGetSymbolAddress(&p, g_error) != cudaSuccess) { cudaGetLastError(); return nullptr; }
   if (dev < kMaxDevices) known[dev] = p;
   return static_cast<uint32_t*>(p);
@@ -58,7 +58,7 @@ int check_cache(const KittyKv8Cache* c, const char* what) {
   if (c->dtype != KITTY_KV8_F16 && c->dtype != KITTY_KV8_BF16)
     return fail(KITTY_ERR_INVALID_ARGUMENT, what, "dtype must be KITTY_KV8_F16 or KITTY_KV8_BF16");
   if (c->pages > 0x7fffffffLL) return fail(KITTY_ERR_INVALID_ARGUMENT, what, "pages must fit int32 page numbers");
-  if (!c->lengths || (c->slots > 0 && (!c->tail_k || !c->tail_v)))
+  if (c->slots > 0 && (!c->lengths || !c->tail_k || !c->tail_v))
     return fail(KITTY_ERR_INVALID_ARGUMENT, what, "NULL lengths or tails");
   if (c->pages > 0 && (!c->key_codes || !c->value_codes || !c->key_scale || !c->value_scale))
     return fail(KITTY_ERR_INVALID_ARGUMENT, what, "NULL pools");

@@ -44,6 +44,7 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kHead = 6.f;           // weights are 2^(score - m + kHead): at most 2^(kHead + kSlack) = 2^14, and
 constexpr float kSlack = 8.f;          // normal in fp16 down to 2^-20 of the one at m
+constexpr float kFar = 1048576.f;      // references beyond this: a product is rounded before the reference is taken off
 constexpr float kUnset = -3.402823466e38f;   // no reference yet: any finite score is far above it
 constexpr int kWarps = 4;              // per CTA
 constexpr int kSetup = 2;              // units (tiles) that beginning and ending a segment count as
@@ -133,10 +134,12 @@ __device__ __forceinline__ Tiles tiles_of(const KittyKv8Cache& c, int len) {
   const int paged = blocks * (c.page_size / kTile);
   return Tiles{paged, paged + (tail + kTile / 2 - 1) / (kTile / 2), tail};
 }
-// Tokens of batch row b: 0 where its slot or its length is out of range.
+// Tokens of batch row b: 0 for padding (a negative slot), and where its slot or its length is
+// out of range.
 __device__ __forceinline__ int tokens_of(const KittyKv8AttentionArgs& a, int b, uint32_t* err = nullptr) {
   const int s = a.seq_map ? a.seq_map[b] : b;
-  if (s < 0 || s >= a.cache.slots) {
+  if (s < 0) return 0;
+  if (s >= a.cache.slots) {
     if (err) dev::flag(err, kErrSlot);
     return 0;
   }
@@ -494,6 +497,7 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
     }
 
     float o[kNT][kOT][4], base[kNT][2], l[kNT][2];   // base: the reference less kHead
+    bool far = false;                               // some reference is beyond kFar
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
 #pragma unroll
@@ -513,7 +517,11 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
         for (int k = 0; k < kGroups; ++k)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            x[k][i] = there(k, i / 2) ? fmaf(s[k][i], i & 1 ? f1_ : f0_, -base[nt][i & 1]) : -INFINITY;
+            const float f = i & 1 ? f1_ : f0_, b = base[nt][i & 1];
+            // The reference is a rounded product.  Far out the rounding is more than the weights'
+            // range, and the products have to be rounded alike.
+            const float y = far ? __fsub_rn(__fmul_rn(s[k][i], f), b) : fmaf(s[k][i], f, -b);
+            x[k][i] = there(k, i / 2) ? y : -INFINITY;
             top = fmaxf(top, x[k][i]);
           }
       };
@@ -532,6 +540,7 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
           best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 16));
           const float now = fmaxf(base[nt][j], best - kHead), alpha = ex2(base[nt][j] - now);
           base[nt][j] = now;
+          far |= fabsf(now) > kFar && now != kUnset;
           l[nt][j] *= alpha;
 #pragma unroll
           for (int i = 0; i < kOT; ++i) {
@@ -539,6 +548,7 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
             o[nt][i][2 + j] *= alpha;
           }
         }
+        far = __any_sync(0xffffffffu, far);
         relative();
       }
 #pragma unroll
@@ -937,17 +947,17 @@ cudaError_t launch_merge(const KittyKv8AttentionArgs& a, const Plan& plan, int h
 // Resident CTAs per SM that a kernel's registers allow (asked once per kernel).
 template <int kDim, int kNT, bool kWhole, bool kBf16, int kCode>
 int resident() {
-  static int known = 0;
-  if (known == 0) {
+  static std::atomic<int> known{0};
+  if (known.load(std::memory_order_relaxed) == 0) {
     int n = 0;
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attention_kernel<kDim, kNT, kWhole, kBf16, kCode>,
                                                       kWarps * 32, 0) != cudaSuccess || n < 1) {
       cudaGetLastError();
       return 1;
     }
-    known = n;
+    known.store(n, std::memory_order_relaxed);
   }
-  return known;
+  return known.load(std::memory_order_relaxed);
 }
 
 // The workspace: the segments' notes, the parts' references and sums, and

@@ -44,9 +44,9 @@ __global__ void __launch_bounds__(kThreads) read_kernel(KittyKv8ReadArgs a, uint
       const int o = a.row_offsets[i];
       if (o < 0 || o > r) {
         bad = kErrRows;
-      } else if (slot < 0 || slot >= c.slots) {
+      } else if (slot >= c.slots) {
         bad = kErrSlot;
-      } else {
+      } else if (slot >= 0) {                 // (a negative slot is padding)
         const int64_t t = first + (r - o);
         const int len = c.lengths[slot];
         if (t < 0 || t >= len || len / G > c.max_pages) {

@@ -120,16 +120,17 @@ __device__ __forceinline__ void quantise_block(const KittyKv8Cache& c, int slot,
   }
 }
 
-// Entry i's slot, its rows [o, o + len) and the tokens it has; false (and flagged) if any
-// of them is out of range, or the slot is an earlier entry's.
+// Entry i's slot, its rows [o, o + len) and the tokens it has; false for padding (a negative
+// slot), and (flagged) if any of them is out of range, or the slot is an earlier entry's.
 __device__ __forceinline__ bool entry_of(const KittyKv8WriteArgs& a, int i, bool first_cta, uint32_t* err, int& slot,
                                          int& o, int& len, int& cached) {
   uint32_t bad = 0;
   slot = a.seq_map ? a.seq_map[i] : i;
+  if (slot < 0) return false;
   o = a.row_offsets ? a.row_offsets[i] : i;
   const int64_t given = a.row_offsets ? int64_t(a.row_offsets[i + 1]) - o : 1;
   len = int(given);
-  if (slot < 0 || slot >= a.cache.slots) {
+  if (slot >= a.cache.slots) {
     bad = kErrSlot;
   } else {
     if (a.seq_map && dev::repeated(a.seq_map, i, slot)) bad = kErrSlot;

@@ -38,10 +38,10 @@ def write_kv8(key: torch.Tensor, value: torch.Tensor, lengths: torch.Tensor, blo
 
     Entry i's rows are ``row_offsets[i]`` .. ``row_offsets[i + 1] - 1`` ((n + 1,) int32;
     without it every entry has one row); they go behind the ``lengths[slot]`` tokens that
-    slot ``seq_map[i]`` ((n,) int32, distinct; without it i) has.  Blocks that fill are quantised into
-    the pages that ``block_table`` holds for them, the rest stays in the tail.  ``lengths``
-    is not changed: add the new tokens before the next call on this cache.  Rows behind
-    the last offset are ignored.
+    slot ``seq_map[i]`` has ((n,) int32, distinct; without it i; negative: padding,
+    skipped).  Blocks that fill are quantised into the pages that ``block_table`` holds for
+    them, the rest stays in the tail.  ``lengths`` is not changed: add the new tokens
+    before the next call on this cache.  Rows behind the last offset are ignored.
     """
     _kv8.ops().write(key, value, lengths, block_table, key_codes, value_codes, key_scale, value_scale, tail_k, tail_v,
                      row_offsets, seq_map)
@@ -56,7 +56,7 @@ def read_kv8(lengths: torch.Tensor, block_table: torch.Tensor, key_codes: torch.
 
     Output rows ``row_offsets[i]`` .. ``row_offsets[i + 1] - 1`` are the tokens of slot
     ``seq_map[i]`` (without it i) from ``first[i]`` (without it 0) on.  Rows behind the
-    last offset, and rows of tokens that the slot does not have, are left as they were
+    last offset, of a negative slot, and of tokens that the slot does not have are left as they were
     (``key_out`` / ``value_out``: the caller's tensors, contiguous).
     """
     return _kv8.ops().read(lengths, block_table, key_codes, value_codes, key_scale, value_scale, tail_k, tail_v,
@@ -72,7 +72,8 @@ def paged_attention_kv8(q: torch.Tensor, lengths: torch.Tensor, block_table: tor
     Row b attends to all ``lengths[slot]`` tokens of slot ``seq_map[b]`` ((B,) int32;
     without it b), query head qh to KV head ``qh // (Hq // H)``; softmax and sums in
     float32, scores scaled by ``sm_scale`` (default 1 / sqrt(D)).  An empty slot gives
-    zeros.  Two launches; the scratch they share is allocated for each call, so calls on
+    zeros, and so does a negative one (a padded batch).  The same call gives the same bits;
+    which tokens are summed together depends on the whole batch's lengths.  Two launches; the scratch they share is allocated for each call, so calls on
     several streams or in several graphs do not meet.
     """
     return _kv8.ops().attention(q, lengths, block_table, key_codes, value_codes, key_scale, value_scale, tail_k, tail_v,

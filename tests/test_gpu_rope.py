@@ -105,3 +105,29 @@ def test_empty_calls():
     q = torch.zeros(0, 4, 64, dtype=FP16, device="cuda")
     qo, ko = K.qk_norm_rope(q, q, torch.zeros(0, dtype=torch.int64, device="cuda"), table)
     assert qo.shape == (0, 4, 64) and ko.shape == (0, 4, 64)
+
+
+def test_norm_without_rotation_and_staged_sizes_in_place():
+    """A table of no columns only normalises; many rows go through the staged form, also in place
+    and with padding rows between."""
+    g = torch.Generator().manual_seed(6)
+    q = torch.randn(5, 3, 64, generator=g).to(BF16).cuda()
+    w = torch.rand(64, generator=g).add(0.5).cuda()
+    pos = torch.arange(5, device="cuda")
+    none = torch.zeros(9, 0, device="cuda")
+    qo, _ = K.qk_norm_rope(q, q, pos, none, w, w)
+    close(qo, q, w, pos, none, 1e-6, False)
+    n = 9000
+    rows = torch.randn(n, 10 * 128, generator=g).to(FP16).cuda()
+    x, y = rows[:, :1024].view(n, 8, 128), rows[:, 1024:].view(n, 2, 128)
+    x0, y0 = x.clone(), y.clone()
+    table = K.rope_table(n, 128, device="cuda")
+    pos = torch.randint(0, n, (n,), generator=g)
+    pos[torch.rand(n, generator=g) < 0.1] = -1
+    pos = pos.cuda()
+    w = torch.rand(128, generator=g).add(0.5).cuda()
+    K.qk_norm_rope(x, y, pos, table, w, w, q_out=x, k_out=y)
+    live = pos >= 0
+    assert torch.equal(x[~live], x0[~live]) and torch.equal(y[~live], y0[~live])
+    close(x[live], x0[live], w, pos[live], table, 1e-6, False)
+    close(y[live], y0[live], w, pos[live], table, 1e-6, False)
