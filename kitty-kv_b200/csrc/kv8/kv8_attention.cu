@@ -301,6 +301,7 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
   const int D = kWhole ? kDim : c.head_dim, G = c.page_size, H = c.num_heads;
   const int g = a.num_q_heads / H;
   const int per_row = H * plan.passes, per_block = G / kTile;
+  dev::wait_for_stream();
   asm volatile("griddepcontrol.launch_dependents;");   // merge_kernel may start to look where its parts will be
   const float fac16 = a.sm_scale * kLog2e;
 
@@ -835,7 +836,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(KittyKv8AttentionA
     note.units = units_of_row<kTile>(a, b);
     note.begin = before * per_row + int64_t(seg) * note.units;
   }
-  asm volatile("griddepcontrol.wait;" ::: "memory");   // attention_kernel is done and its parts are visible
+  dev::wait_for_stream();                              // attention_kernel is done and its parts are visible
   if (b >= a.batch || heads <= 0) return;
   if (note.units == -2) {
     note = plan.notes[segment];
@@ -927,21 +928,14 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(KittyKv8AttentionA
   }
 }
 
-// merge_kernel behind attention_kernel, as its programmatic dependent: it is launched while
-// the other runs and waits in front of the first part that it reads.
+// merge_kernel starts while attention_kernel runs and waits in front of the first part.
 template <int kTile, bool kBf16, int kTeam>
-cudaError_t launch_merge(const KittyKv8AttentionArgs& a, const Plan& plan, int heads_each, cudaStream_t s) {
-  const unsigned teams = unsigned(a.batch) * a.cache.num_heads * plan.passes * ((plan.pass_heads + heads_each - 1) / heads_each);
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((teams + kMergeThreads / kTeam - 1) / (kMergeThreads / kTeam));
-  cfg.blockDim = kMergeThreads;
-  cfg.stream = s;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, merge_kernel<kTile, kBf16, kTeam>, a, plan, heads_each);
+int launch_merge(const KittyKv8AttentionArgs& a, const Plan& plan, int heads_each, cudaStream_t s) {
+  const unsigned teams =
+      unsigned(a.batch) * a.cache.num_heads * plan.passes * ((plan.pass_heads + heads_each - 1) / heads_each);
+  const dim3 grid((teams + kMergeThreads / kTeam - 1) / (kMergeThreads / kTeam));
+  return launch_dependent("kv8_attention (merge)", merge_kernel<kTile, kBf16, kTeam>, grid, kMergeThreads, 0, s, a, plan,
+                          heads_each);
 }
 
 // Resident CTAs per SM that a kernel's registers allow (asked once per kernel).
@@ -981,18 +975,16 @@ int launch(const KittyKv8AttentionArgs& a, Plan plan, uint32_t* err, cudaStream_
   if (bytes) { *bytes = need; return KITTY_OK; }
   if (a.workspace_bytes < need)
     return fail(KITTY_ERR_WORKSPACE, "kv8_attention", "workspace smaller than kitty_kv8_attention_workspace_size()");
-  attention_kernel<kDim, kNT, kWhole, kBf16, kCode><<<grid, kWarps * 32, 0, s>>>(a, plan, err);
-  const int rc = check_launch("kv8_attention");
+  const int rc = launch_dependent("kv8_attention", attention_kernel<kDim, kNT, kWhole, kBf16, kCode>, dim3(unsigned(grid)),
+                                  kWarps * 32, 0, s, a, plan, err);
   if (rc != KITTY_OK) return rc;
   // Many warps to a segment: a CTA joins a head.  Otherwise a warp joins as many heads as it has
   // lanes for: of 256 mixed lengths, 2048 segments of 5 heads, in 58.5 us all told (one head a
   // warp 60.5, all five 60.8).
   const int64_t segments = int64_t(a.batch) * a.cache.num_heads * plan.passes;
   const int heads_each = std::min(std::max(1, 128 / a.cache.head_dim), plan.pass_heads);
-  const cudaError_t e = segments * 32 < plan.warps
-                            ? launch_merge<kTileOf<kDim>, kBf16, kMergeThreads>(a, plan, 1, s)
-                            : launch_merge<kTileOf<kDim>, kBf16, 32>(a, plan, heads_each, s);
-  return e == cudaSuccess ? KITTY_OK : fail(KITTY_ERR_CUDA, "kv8_attention (merge)", cudaGetErrorString(e));
+  return segments * 32 < plan.warps ? launch_merge<kTileOf<kDim>, kBf16, kMergeThreads>(a, plan, 1, s)
+                                    : launch_merge<kTileOf<kDim>, kBf16, 32>(a, plan, heads_each, s);
 }
 
 template <int kDim, bool kWhole, bool kBf16, int kCode>

@@ -28,10 +28,35 @@ int sm_count();                       // of the current device
 uint32_t* error_word();               // device address of the sticky bits on the current device (host call)
 int check_cache(const KittyKv8Cache* c, const char* what);
 
+// Launch as a programmatic dependent of whatever is before it on the stream: the launch itself
+// overlaps the end of that, and the kernel waits (dev::wait_for_stream, before it touches
+// memory) until it is done.  Between the short kernels of a decode step that is 1 to 2 us:
+// eager calls of 256 single-token writes 6.1 -> 4.6 us, of a read of 4137 tokens 8.2 -> 6.5, of
+// attention over 4133 tokens 14.3 -> 12.4.
+template <typename... Params, typename... Args>
+int launch_dependent(const char* what, void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t s,
+                     Args... args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
+  return e == cudaSuccess ? KITTY_OK : fail(KITTY_ERR_CUDA, what, cudaGetErrorString(e));
+}
+
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 namespace dev {
+
+// What was before this kernel on its stream is done, and its writes are visible.
+__device__ __forceinline__ void wait_for_stream() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __forceinline__ void flag(uint32_t* word, uint32_t bits) { atomicOr(word, bits); }
 

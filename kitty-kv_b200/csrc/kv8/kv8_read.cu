@@ -23,6 +23,7 @@ struct RowAt {
 template <bool kBf16, int kCode, int kRows>
 __global__ void __launch_bounds__(kThreads) read_kernel(KittyKv8ReadArgs a, uint32_t* err) {
   __shared__ RowAt s_row[kRows];
+  dev::wait_for_stream();
   const KittyKv8Cache& c = a.cache;
   const int G = c.page_size, D = c.head_dim, H = c.num_heads;
   const int64_t r0 = int64_t(blockIdx.x) * kRows;
@@ -120,10 +121,10 @@ template <bool kBf16, int kCode>
 int launch(const KittyKv8ReadArgs& a, uint32_t* err, cudaStream_t s) {
   // Many rows: 32 a CTA, which finds their pages once.  Few: 8, so that every SM has some.
   if (int64_t(a.rows) * a.cache.num_heads * a.cache.head_dim > kManyValues * sm_count())
-    read_kernel<kBf16, kCode, 32><<<unsigned((int64_t(a.rows) + 31) / 32), kThreads, 0, s>>>(a, err);
-  else
-    read_kernel<kBf16, kCode, 8><<<unsigned((int64_t(a.rows) + 7) / 8), kThreads, 0, s>>>(a, err);
-  return check_launch("kv8_read");
+    return launch_dependent("kv8_read", read_kernel<kBf16, kCode, 32>, dim3(unsigned((int64_t(a.rows) + 31) / 32)),
+                            kThreads, 0, s, a, err);
+  return launch_dependent("kv8_read", read_kernel<kBf16, kCode, 8>, dim3(unsigned((int64_t(a.rows) + 7) / 8)), kThreads, 0,
+                          s, a, err);
 }
 
 }  // namespace

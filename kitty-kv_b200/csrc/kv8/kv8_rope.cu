@@ -30,6 +30,7 @@ __device__ __forceinline__ void copy_async(uint4* dst, const void* src) {
 template <bool kBf16, int kLanes, bool kInter, int kPasses, int kStages>
 __global__ void __launch_bounds__(kThreads, kCtas) qk_norm_rope_kernel(KittyQkNormRopeArgs a, RopeShape sh, uint32_t* err) {
   constexpr int kRows = 32 / kLanes;                       // rows that a warp holds at once
+  dev::wait_for_stream();
   const int lane = threadIdx.x & 31, j = lane % kLanes;
   const int64_t warps = int64_t(gridDim.x) * (kThreads / 32) / sh.chunks * sh.chunks;
   const int64_t gw = int64_t(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
@@ -190,8 +191,7 @@ int launch(const KittyQkNormRopeArgs& a, uint32_t* err, cudaStream_t s) {
   if (kBytes > 48 * 1024 &&
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes) != cudaSuccess)
     return check_launch("qk_norm_rope");
-  kernel<<<unsigned(grid), kThreads, kBytes, s>>>(a, sh, err);
-  return check_launch("qk_norm_rope");
+  return launch_dependent("qk_norm_rope", kernel, dim3(unsigned(grid)), kThreads, kBytes, s, a, sh, err);
 }
 
 template <bool kBf16, int kLanes>

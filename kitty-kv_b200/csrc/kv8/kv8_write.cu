@@ -151,6 +151,7 @@ __device__ __forceinline__ const uint16_t* row_of(const void* base, int64_t row,
 template <bool kBf16, int kCode, int kPer>
 __global__ void __launch_bounds__(kThreads, kMinCtas) write_kernel(KittyKv8WriteArgs a, uint32_t* err) {
   __shared__ uint32_t s_top[2][kThreads / 32];
+  dev::wait_for_stream();
   const KittyKv8Cache& c = a.cache;
   const int G = c.page_size, D = c.head_dim;
   const int item = blockIdx.x / c.num_heads, h = blockIdx.x - item * c.num_heads;
@@ -201,6 +202,7 @@ __global__ void __launch_bounds__(kThreads, kMinCtas) write_kernel(KittyKv8Write
 template <bool kBf16, int kCode, int kPer>
 __global__ void __launch_bounds__(kThreads, kMinCtas) write_step_kernel(KittyKv8WriteArgs a, uint32_t* err) {
   __shared__ uint32_t s_top[2][kThreads / 32];
+  dev::wait_for_stream();
   const KittyKv8Cache& c = a.cache;
   const int G = c.page_size, D = c.head_dim, H = c.num_heads, per = vecs_of_row<kPer>(D);
   const int groups = (a.n + kStepEntries - 1) / kStepEntries;
@@ -252,9 +254,9 @@ int launch(const KittyKv8WriteArgs& a, uint32_t* err, cudaStream_t s) {
   const int64_t ctas = a.row_offsets ? (int64_t(a.n) + a.rows / a.cache.page_size) * H
                                      : (int64_t(a.n) + kStepEntries - 1) / kStepEntries * H + a.n;
   if (ctas > 0x7fffffff) return fail(KITTY_ERR_UNSUPPORTED, "kv8_write", "too many rows times heads for one launch");
-  if (a.row_offsets) write_kernel<kBf16, kCode, kPer><<<unsigned(ctas), kThreads, 0, s>>>(a, err);
-  else write_step_kernel<kBf16, kCode, kPer><<<unsigned(ctas), kThreads, 0, s>>>(a, err);
-  return check_launch("kv8_write");
+  const dim3 grid{unsigned(ctas)};
+  return a.row_offsets ? launch_dependent("kv8_write", write_kernel<kBf16, kCode, kPer>, grid, kThreads, 0, s, a, err)
+                       : launch_dependent("kv8_write", write_step_kernel<kBf16, kCode, kPer>, grid, kThreads, 0, s, a, err);
 }
 
 template <bool kBf16, int kCode>
