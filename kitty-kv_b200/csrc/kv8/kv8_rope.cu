@@ -14,7 +14,10 @@ namespace kitty8 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kCtas = 2;       // resident on an SM
+// CTAs resident on an SM: a warp with one row for each lane group needs half the registers and
+// has a quarter of the bytes in flight.
+template <int kPasses>
+constexpr int kCtas = kPasses == 1 ? 3 : 2;
 
 struct RopeShape {
   int q_chunks, chunks;        // warps per token: ceil(heads / rows of a warp), queries first
@@ -28,7 +31,7 @@ __device__ __forceinline__ void copy_async(uint4* dst, const void* src) {
 // kPasses: rows per lane group and token, which share the table values; kStages: tokens of
 // a warp in flight in shared memory, 0: no stage, the rows go to registers.
 template <bool kBf16, int kLanes, bool kInter, int kPasses, int kStages>
-__global__ void __launch_bounds__(kThreads, kCtas) qk_norm_rope_kernel(KittyQkNormRopeArgs a, RopeShape sh, uint32_t* err) {
+__global__ void __launch_bounds__(kThreads, kCtas<kPasses>) qk_norm_rope_kernel(KittyQkNormRopeArgs a, RopeShape sh, uint32_t* err) {
   constexpr int kRows = 32 / kLanes;                       // rows that a warp holds at once
   dev::wait_for_stream();
   const int lane = threadIdx.x & 31, j = lane % kLanes;
@@ -183,7 +186,7 @@ int launch(const KittyQkNormRopeArgs& a, uint32_t* err, cudaStream_t s) {
   sh.chunks = sh.q_chunks + (a.num_k_heads + kHeads - 1) / kHeads;
   const int64_t warps = int64_t(a.rows) * sh.chunks, per = kThreads / 32;
   // at least one warp for each chunk of heads, at most what the card holds at once
-  const int64_t most = std::max<int64_t>(int64_t(sm_count()) * kCtas, (sh.chunks + per - 1) / per);
+  const int64_t most = std::max<int64_t>(int64_t(sm_count()) * kCtas<kPasses>, (sh.chunks + per - 1) / per);
   const int64_t grid = std::min((warps + per - 1) / per, most);
   constexpr int kBytes = kStages * (kThreads / 32) * kPasses * 2 * 32 * 16;
   const auto kernel = a.interleaved ? qk_norm_rope_kernel<kBf16, kLanes, true, kPasses, kStages>
@@ -199,9 +202,11 @@ int launch_size(const KittyQkNormRopeArgs& a, uint32_t* err, cudaStream_t s) {
   // Stages pay where a resident warp has more than one token (40 heads of 128: 8.0 against
   // 9.3 us for 1024 tokens, 32 against 40 for 8192, 114 against 119 for 32768) and cost where it
   // has one (301 tokens of 72 heads: 6.3 and 5.1 us).
+  // With no more heads than a warp has lane groups, rows behind the first would be empty.
+  if (std::max(a.num_q_heads, a.num_k_heads) <= 32 / kLanes) return launch<kBf16, kLanes, 1, 0>(a, err, s);
   constexpr int kStaged = 4, kHeads = 32 / kLanes * kStaged;
   const int64_t chunks = (a.num_q_heads + kHeads - 1) / kHeads + (a.num_k_heads + kHeads - 1) / kHeads;
-  return a.rows * chunks > int64_t(sm_count()) * kCtas * (kThreads / 32) ? launch<kBf16, kLanes, kStaged, 2>(a, err, s)
+  return a.rows * chunks > int64_t(sm_count()) * kCtas<kStaged> * (kThreads / 32) ? launch<kBf16, kLanes, kStaged, 2>(a, err, s)
                                                                          : launch<kBf16, kLanes, 2, 0>(a, err, s);
 }
 
