@@ -95,6 +95,10 @@ __global__ void __launch_bounds__(kThreads, kCtas<kPasses>) qk_norm_rope_kernel(
     }
     if constexpr (kStages > 0) asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  // The copies of the token at hand are there; only the later ones' may be on their way.
+  auto arrive = [&]() {
+    if constexpr (kStages > 0) asm volatile("cp.async.wait_group %0;" :: "n"(kStages - 1) : "memory");
+  };
   auto position = [&](int64_t t) {
     return t >= a.rows ? int64_t(-1)
            : a.positions64 ? static_cast<const int64_t*>(a.positions)[t]
@@ -109,9 +113,9 @@ __global__ void __launch_bounds__(kThreads, kCtas<kPasses>) qk_norm_rope_kernel(
     next = position(t + step);
     if constexpr (kStages > 0) fetch(t + (kStages - 1) * step, stage == 0 ? kStages - 1 : stage - 1);
     else fetch(t, 0);
-    if (pos < 0) continue;                                  // a padding row
-    if (pos >= a.table_rows) {
-      if (lane == 0) dev::flag(err, kErrPosition);
+    if (pos < 0 || pos >= a.table_rows) {                   // a padding row, or none of the table
+      if (pos >= 0 && lane == 0) dev::flag(err, kErrPosition);
+      arrive();                                             // before another copy goes to this stage
       continue;
     }
     float cs[8], sn[8];
@@ -120,12 +124,12 @@ __global__ void __launch_bounds__(kThreads, kCtas<kPasses>) qk_norm_rope_kernel(
       const float4* ts = reinterpret_cast<const float4*>(a.table + pos * a.rot + a.rot / 2 + 8 * j);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float4 u = __ldg(tc + i), v = __ldg(ts + i);
+        const float4 u = tc[i], v = ts[i];
         cs[4 * i] = u.x; cs[4 * i + 1] = u.y; cs[4 * i + 2] = u.z; cs[4 * i + 3] = u.w;
         sn[4 * i] = v.x; sn[4 * i + 1] = v.y; sn[4 * i + 2] = v.z; sn[4 * i + 3] = v.w;
       }
     }
-    if constexpr (kStages > 0) asm volatile("cp.async.wait_group %0;" :: "n"(kStages - 1) : "memory");
+    arrive();
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
       const int h = h0 + p * kRows;

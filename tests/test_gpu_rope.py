@@ -131,3 +131,22 @@ def test_norm_without_rotation_and_staged_sizes_in_place():
     assert torch.equal(x[~live], x0[~live]) and torch.equal(y[~live], y0[~live])
     close(x[live], x0[live], w, pos[live], table, 1e-6, False)
     close(y[live], y0[live], w, pos[live], table, 1e-6, False)
+
+
+def test_padding_between_staged_rows_again_and_again():
+    """A row that is skipped leaves its copy in flight: the next copy to that place has to wait
+    for it.  Half of the rows are padding, in runs of every length, and each call is checked."""
+    g = torch.Generator().manual_seed(7)
+    n = 12000
+    x = torch.randn(n, 16, 128, generator=g).to(BF16).cuda()
+    y = torch.randn(n, 4, 128, generator=g).to(BF16).cuda()
+    table = K.rope_table(n, 128, device="cuda")
+    pos = torch.randint(0, n, (n,), generator=g)
+    want = K.qk_norm_rope(x, y, pos.cuda(), table)
+    for i in range(20):
+        some = pos.clone()
+        some[torch.rand(n, generator=g) < 0.5] = -1
+        some[i * 100:i * 100 + 5000] = -1
+        live = (some >= 0).cuda()
+        got = K.qk_norm_rope(x, y, some.cuda(), table)
+        assert torch.equal(got[0][live], want[0][live]) and torch.equal(got[1][live], want[1][live])
