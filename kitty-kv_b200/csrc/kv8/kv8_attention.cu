@@ -50,7 +50,6 @@ constexpr int kWarps = 4;              // per CTA
 constexpr int kSetup = 2;              // units (tiles) that beginning and ending a segment count as
 constexpr int kAhead = 4;              // tiles that a prefetch asks for
 constexpr int kMergeThreads = 256;
-constexpr int kBatch = 8;              // parts whose loads merge_kernel has in flight
 
 // What attention_kernel leaves about a segment for merge_kernel.
 struct alignas(16) Note {
@@ -66,15 +65,17 @@ struct Plan {
   Note* notes;                         // [segments + 1], the last holding the units of a slice
 };
 
+// Read once, past L1.  (Not as read-only data: this kernel may have been launched before the
+// one that writes it was done.)
 __device__ __forceinline__ uint4 ld_stream(const void* p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
 __device__ __forceinline__ uint2 ld_stream2(const void* p) {
   uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
   return v;
 }
 __device__ __forceinline__ float ex2(float x) {
@@ -268,7 +269,7 @@ __device__ __forceinline__ Place locate(const KittyKv8AttentionArgs& a, int per_
   return r;
 }
 
-// Whether all warps of the CTA that holds warp w work on the segment [begin, end) only.
+// Whether all warps of a CTA work on tiles of the segment [begin, end) only.
 __device__ __forceinline__ bool cta_inside(int64_t cta, int64_t per_warp, int64_t begin, int64_t end) {
   return cta * kWarps * per_warp >= begin + kSetup && (cta + 1) * kWarps * per_warp <= end;
 }
@@ -381,7 +382,7 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
         for (int jj = 0; jj < kKC; ++jj)
           kr[r * kKC + jj] = kWhole || 64 * jj + 16 * lc < D ? ld_stream(p + r * 8 * D + 64 * jj)
                                                              : make_uint4(0, 0, 0, 0);
-      ks = __ldg(c.key_scale + int64_t(page) * H + h);
+      ks = c.key_scale[int64_t(page) * H + h];
     };
     auto load_tail_keys = [&](int t) {
       const int tok = (t - tl.paged) * kTailTile + lr;
@@ -416,7 +417,7 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
               v[0] = u.x; v[1] = u.y;
             }
           }
-      vs = __ldg(c.value_scale + int64_t(page) * H + h);
+      vs = c.value_scale[int64_t(page) * H + h];
     };
     auto load_tail_values = [&](int t) {
       // rows behind the tail's end may hold anything: they read as zero
@@ -807,6 +808,7 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
 // Otherwise the team is a warp, for `heads_each` heads.
 template <int kTile, bool kBf16, int kTeam>
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(KittyKv8AttentionArgs a, Plan plan, int heads_each) {
+  constexpr int kBatch = kTeam == 32 ? 4 : 8;          // parts whose loads are in flight
   __shared__ float4 s_sum[kTeam == 32 ? 1 : kTeam];
   __shared__ float s_l[kTeam == 32 ? 1 : kTeam], s_m[kTeam == 32 ? 1 : kTeam];
   const KittyKv8Cache& c = a.cache;
@@ -1063,5 +1065,7 @@ extern "C" int kitty_kv8_attention(const KittyKv8AttentionArgs* a, void* stream)
     return fail(KITTY_ERR_WORKSPACE, what, "workspace missing or not 16-byte aligned");
   uint32_t* err = error_word();
   if (!err) return fail(KITTY_ERR_CUDA, what, "no CUDA device");
-  return dispatch(*a, err, as_stream(stream), nullptr);
+  KittyKv8AttentionArgs args = *a;
+  if (args.cache.pages == 0) args.cache.max_pages = 0;     // without a page 0 to stand for a missing one, tails only
+  return dispatch(args, err, as_stream(stream), nullptr);
 }

@@ -55,7 +55,8 @@ inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_
 
 namespace dev {
 
-// What was before this kernel on its stream is done, and its writes are visible.
+// What was before this kernel on its stream is done, and its writes are visible (to loads that
+// are not marked read-only).
 __device__ __forceinline__ void wait_for_stream() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __forceinline__ void flag(uint32_t* word, uint32_t bits) { atomicOr(word, bits); }
@@ -128,7 +129,7 @@ __device__ __forceinline__ float4 decode4(uint32_t w) {
 
 // Number of the n values of the ascending array a that are <= v, by the whole warp: each
 // step looks at 32 evenly spaced values at once.  Any contents end within the bounds.
-__device__ __forceinline__ int count_le(const int32_t* __restrict__ a, int n, int v) {
+__device__ __forceinline__ int count_le(const int32_t* a, int n, int v) {
   const int lane = threadIdx.x & 31;
   int lo = 0, len = n;                 // the answer lies in [lo, lo + len]
   while (len > 0) {
@@ -145,7 +146,7 @@ __device__ __forceinline__ int count_le(const int32_t* __restrict__ a, int n, in
 }
 
 // Whether entry i's slot is given by an earlier entry too (by the whole warp).
-__device__ __forceinline__ bool repeated(const int32_t* __restrict__ seq_map, int i, int slot) {
+__device__ __forceinline__ bool repeated(const int32_t* seq_map, int i, int slot) {
   bool hit = false;
   for (int j = threadIdx.x & 31; j < i; j += 32) hit |= seq_map[j] == slot;
   return __any_sync(0xffffffffu, hit);

@@ -90,10 +90,10 @@ __global__ void __launch_bounds__(kThreads) read_kernel(KittyKv8ReadArgs a, uint
           page[k] = at.page;
           if (at.page >= 0) {
             const int64_t scale = int64_t(at.page) * H + h;
-            w[k][0] = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(c.key_codes) + off));
-            w[k][1] = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(c.value_codes) + off));
-            sc[k][0] = __ldg(c.key_scale + scale);
-            sc[k][1] = __ldg(c.value_scale + scale);
+            w[k][0] = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(c.key_codes) + off);
+            w[k][1] = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(c.value_codes) + off);
+            sc[k][0] = c.key_scale[scale];
+            sc[k][1] = c.value_scale[scale];
           } else if (at.page == -1) {
             static_cast<uint4*>(a.key)[to] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.tail_k) + off);
             static_cast<uint4*>(a.value)[to] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.tail_v) + off);

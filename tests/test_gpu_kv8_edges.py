@@ -61,6 +61,22 @@ def test_cache_without_pages_and_table_with_strided_rows():
     check_attention(m, 3, q=q, got=got)
 
 
+def test_an_empty_pool_has_tails_only():
+    """Lengths that ask for pages of a pool that has none: flagged, no tokens, no page touched."""
+    m = CacheModel(3, 1, 64, 32, E4M3, BF16, pages=0, table_width=2, seed=12)
+    m.append(0, m.new_rows(9), m.new_rows(9))
+    m.fill_arrays()
+    lens = m.lens()
+    lens[1], lens[2] = 40, 64
+    q = torch.randn(3, 2, 64, generator=m.g).to(BF16).cuda()
+    got = K.paged_attention_kv8(q, lens, *m.arrays())
+    assert K.kv8_error_flags() == 1 << 4 and not got[1:].any()
+    check_attention(m, 2, rows=[0], q=q[:1], got=got[:1])
+    k = torch.full((40, 1, 64), 3.0, dtype=BF16, device="cuda")
+    K.read_kv8(lens, *m.arrays(), i32([0, 0, 40, 40]), 40, key_out=k)
+    assert K.kv8_error_flags() == 1 << 1 and (k[:32] == 3).all() and not (k[32:] == 3).any()
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("code", [E4M3, INT8])
 def test_scores_far_from_zero(code, dtype):
