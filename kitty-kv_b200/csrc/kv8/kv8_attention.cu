@@ -514,21 +514,22 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
     auto weigh = [&](auto& s, int nt, float f0_, float f1_, auto there) {
       constexpr int kGroups = sizeof(s) / sizeof(s[0]);
       float x[kGroups][4], top = -INFINITY;
-      auto relative = [&]() {
+      auto relative = [&](bool rounded) {
 #pragma unroll
         for (int k = 0; k < kGroups; ++k)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float f = i & 1 ? f1_ : f0_, b = base[nt][i & 1];
-            // The reference is a rounded product.  Far out the rounding is more than the weights'
-            // range, and the products have to be rounded alike.
-            const float y = far ? __fsub_rn(__fmul_rn(s[k][i], f), b) : fmaf(s[k][i], f, -b);
+            const float y = rounded ? __fsub_rn(__fmul_rn(s[k][i], f), b) : fmaf(s[k][i], f, -b);
             x[k][i] = there(k, i / 2) ? y : -INFINITY;
             top = fmaxf(top, x[k][i]);
           }
       };
-      relative();
-      if (!__all_sync(0xffffffffu, top <= kHead + kSlack)) {   // a score far above the reference (or none yet, or NaN)
+      relative(false);
+      // A score far above the reference, none yet, or NaN; or a reference so far out that its
+      // rounding (it is a rounded product) is more than the weights' range, where the products
+      // have to be rounded alike.
+      if (far || !__all_sync(0xffffffffu, top <= kHead + kSlack)) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           float best = -INFINITY;
@@ -551,7 +552,8 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
           }
         }
         far = __any_sync(0xffffffffu, far);
-        relative();
+        if (far) relative(true);
+        else relative(false);
       }
 #pragma unroll
       for (int k = 0; k < kGroups; ++k)
