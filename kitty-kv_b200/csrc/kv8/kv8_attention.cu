@@ -136,15 +136,16 @@ __device__ __forceinline__ Tiles tiles_of(const KittyKv8Cache& c, int len) {
   return Tiles{paged, paged + (tail + kTile / 2 - 1) / (kTile / 2), tail};
 }
 // Tokens of batch row b: 0 for padding (a negative slot), and where its slot or its length is
-// out of range.
+// out of range.  (From L2: merge_kernel asks before it has waited, and the SM's L1 may hold
+// what was there before the last kernel on the stream.)
 __device__ __forceinline__ int tokens_of(const KittyKv8AttentionArgs& a, int b, uint32_t* err = nullptr) {
-  const int s = a.seq_map ? a.seq_map[b] : b;
+  const int s = a.seq_map ? __ldcg(a.seq_map + b) : b;
   if (s < 0) return 0;
   if (s >= a.cache.slots) {
     if (err) dev::flag(err, kErrSlot);
     return 0;
   }
-  const int len = a.cache.lengths[s];
+  const int len = __ldcg(a.cache.lengths + s);
   if (len >= 0 && len / a.cache.page_size <= a.cache.max_pages) return len;
   if (err) dev::flag(err, kErrLength);
   return 0;

@@ -298,6 +298,7 @@ extern "C" int kitty_kv8_write(const KittyKv8WriteArgs* a, void* stream) {
   const int rc = check_cache(&a->cache, what);
   if (rc != KITTY_OK) return rc;
   if (a->n < 0 || a->rows < 0) return fail(KITTY_ERR_INVALID_ARGUMENT, what, "negative size");
+  if (a->n > 0x7fffff00) return fail(KITTY_ERR_UNSUPPORTED, what, "too many entries");     // n + 32 is an int
   if (!a->row_offsets && a->n != a->rows)
     return fail(KITTY_ERR_INVALID_ARGUMENT, what, "without row_offsets there is one row for each entry");
   if (!a->seq_map && a->n > a->cache.slots)

@@ -157,6 +157,105 @@ def test_overlapping_calls_on_several_streams():
         assert all(torch.equal(w, o) for o in outs)
 
 
+def test_output_in_the_place_of_the_queries():
+    """Rows whose segments are stored by one warp, and rows joined from many parts."""
+    for lens, hq in (([9000, 5, 0], 8), ([9000, 5, 0], 40), ([40 + i for i in range(200)], 4)):
+        m = filled(lens, 2, 64, 32, E4M3, BF16, seed=len(lens) + hq)
+        q = torch.randn(len(lens), hq, 64, generator=m.g).to(BF16).cuda()
+        want = K.paged_attention_kv8(q, m.lens(), *m.arrays())
+        assert K.paged_attention_kv8(q, m.lens(), *m.arrays(), out=q) is q and torch.equal(q, want)
+
+
+@pytest.mark.parametrize("n", [1, 30, 31, 32, 33, 63, 64, 65, 500])
+@pytest.mark.parametrize("heads", [1, 8])
+def test_read_of_many_entries_most_of_them_empty(n, heads):
+    """Runs of entries without rows, longer than a warp, between and behind entries with some."""
+    m = filled([70, 33, 64], heads, 64, 32, INT8, FP16, seed=n)
+    g = torch.Generator().manual_seed(n)
+    counts = torch.where(torch.rand(n, generator=g) < 0.1, torch.randint(1, 30, (n,), generator=g), 0)
+    counts[-1] = 3
+    slots, first = torch.randint(0, 3, (n,), generator=g), torch.randint(0, 4, (n,), generator=g)
+    offsets = [2] + (counts.cumsum(0) + 2).tolist()
+    rows = offsets[-1] + 2
+    ko = torch.full((rows, heads, 64), 9.0, dtype=FP16, device="cuda")
+    k, v = K.read_kv8(m.lens(), *m.arrays(), i32(offsets), rows, first=i32(first.tolist()), seq_map=i32(slots.tolist()),
+                      key_out=ko)
+    want = [[torch.full((2, heads, 64), 9.0, dtype=FP16)], []]
+    for x in range(2):
+        for c, s, f in zip(counts.tolist(), slots.tolist(), first.tolist()):
+            want[x].append(m.truth(s)[x][:, f:f + c].transpose(0, 1).float().to(FP16))
+    want[0].append(want[0][0])
+    assert torch.equal(k.cpu(), torch.cat(want[0])) and torch.equal(v[2:-2].cpu(), torch.cat(want[1]))
+    assert K.kv8_error_flags() == 0
+
+
+def test_in_a_graph_behind_copies_fills_and_other_streams():
+    """Each operator captured behind what is not a kernel (a copy, a fill), as the first of its
+    graph, and behind two streams that meet."""
+    m = filled([300, 31, 0, 95], 2, 128, 32, E4M3, BF16, seed=50)
+    m.table[1, 0], m.table[3, 2] = m.free.pop(), m.free.pop()          # of the blocks that a token completes
+    n, arrays = m.lens(), m.arrays()
+    q0, k0 = (torch.randn(4, h, 128, generator=m.g).to(BF16).cuda() for h in (8, 2))
+    table, pos, off = K.rope_table(512, 128, device="cuda"), i32([300, 31, 0, 95]), i32([0, 300, 331, 331, 426])
+    lens, q, k = n.clone(), q0.clone(), k0.clone()
+    mutable = arrays[1:]
+    start = [t.clone() for t in mutable]
+
+    def call(what):
+        if what == "rope":
+            return K.qk_norm_rope(q, k, pos, table)
+        if what == "write":
+            K.write_kv8(k, k, lens, *arrays)
+            return mutable
+        if what == "read":
+            return K.read_kv8(lens, *arrays, off, 426)
+        return (K.paged_attention_kv8(q, lens, *arrays),)
+
+    def before(how):
+        if how == "copies":
+            lens.copy_(n), q.copy_(q0), k.copy_(k0)
+        elif how == "fills":
+            lens.zero_(), q.zero_(), k.zero_()
+        elif how == "streams":
+            main, side = torch.cuda.current_stream(), torch.cuda.Stream()
+            side.wait_stream(main)
+            with torch.cuda.stream(side):
+                k.mul_(2)
+                lens.copy_(n)
+            q.mul_(2)
+            main.wait_stream(side)
+
+    def same(a, b):
+        return all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(a, b))
+
+    for how in ("first", "copies", "fills", "streams"):
+        for what in ("rope", "write", "read", "attention"):
+            def set_up():
+                for t, s in zip(mutable, start):
+                    t.copy_(s)
+                lens.copy_(n), q.copy_(q0), k.copy_(k0)
+                torch.cuda.synchronize()
+            set_up()
+            before(how)
+            torch.cuda.synchronize()
+            want = [t.clone() for t in call(what)]
+            flags = K.kv8_error_flags()                # (rows of emptied slots are none that can be read)
+            graph = torch.cuda.CUDAGraph()
+            set_up()
+            with torch.cuda.graph(graph):
+                before(how)
+                got = call(what)
+            for _ in range(3):
+                if what == "read":
+                    for t, w in zip(got, want):
+                        t.copy_(w)                     # rows that are not read are left as they were
+                set_up()
+                graph.replay()
+                torch.cuda.synchronize()
+                assert same(got, want), (how, what)
+            assert K.kv8_error_flags() == flags == (1 << 4 if how == "fills" and what == "read" else 0)
+
+
 FIRST = """
 import sys
 sys.path[:0] = [{root!r}, {root!r} + "/kitty-kv_b200"]
