@@ -1,8 +1,9 @@
 // Reading the cache back to 16-bit rows.
 //
 // A CTA takes kRows output rows (tokens, all heads).  Its first warp finds each row's slot
-// and page by a search of the row offsets and leaves them in shared memory; then every
-// thread turns eight codes of keys and of values (8 bytes each) into 16-byte stores,
+// and page and leaves them in shared memory: 32 entries' offsets, slots and first tokens are
+// loaded at once and searched by shuffles (a search in memory is a chain of loads, 5 for 24
+// entries), then the row's page and its slot's length, also at once.  Then every thread turns eight codes of keys and of values (8 bytes each) into 16-byte stores,
 // contiguous over the row, at the same place of one row after another.  Bound by HBM: 1
 // byte read and 2 written a value.
 #include "kv8_common.cuh"
@@ -28,44 +29,58 @@ __global__ void __launch_bounds__(kThreads) read_kernel(KittyKv8ReadArgs a, uint
   const int G = c.page_size, D = c.head_dim, H = c.num_heads;
   const int64_t r0 = int64_t(blockIdx.x) * kRows;
   const int count = int(min(int64_t(kRows), a.rows - r0));
-  if (int(threadIdx.x) < count) {
-    const int r = int(r0) + threadIdx.x;
-    int lo = 0, hi = a.n + 1;            // how many offsets are <= r (any contents end within the bounds)
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (a.row_offsets[mid] <= r) lo = mid + 1;
-      else hi = mid;
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x, r = int(r0) + min(lane, count - 1);
+    const int at0 = a.n < 32 ? 0 : max(dev::count_le(a.row_offsets, a.n + 1, int(r0)) - 1, 0);
+    const int e = at0 + lane;            // this lane's entry of the window
+    const int offset = e <= a.n ? a.row_offsets[e] : 0x7fffffff;
+    const int window_slot = e < a.n && a.seq_map ? a.seq_map[e] : e, window_first = e < a.n && a.first ? a.first[e] : 0;
+    int lo = 0;                          // how many of the window's offsets are <= r
+#pragma unroll
+    for (int step = 16; step > 0; step >>= 1)
+      if (__shfl_sync(0xffffffffu, offset, lo + step - 1) <= r) lo += step;
+    if (__shfl_sync(0xffffffffu, offset, lo) <= r) ++lo;          // (31 of them, or 32)
+    const int from = max(lo - 1, 0);
+    int i = at0 + lo - 1, o = __shfl_sync(0xffffffffu, offset, from), slot = __shfl_sync(0xffffffffu, window_slot, from),
+        first = __shfl_sync(0xffffffffu, window_first, from);
+    if (lo == 32 && at0 + 32 <= a.n) {   // the row is behind the window: many entries of no or few rows
+      int hi = a.n + 1;
+      lo = at0 + 32;
+      while (lo < hi) {
+        const int mid = lo + (hi - lo) / 2;
+        if (a.row_offsets[mid] <= r) lo = mid + 1;
+        else hi = mid;
+      }
+      i = lo - 1;
+      o = a.row_offsets[i];
+      if (i < a.n) {
+        slot = a.seq_map ? a.seq_map[i] : i;
+        first = a.first ? a.first[i] : 0;
+      }
     }
-    const int i = lo - 1;
     RowAt at{0, -2};
     uint32_t bad = 0;
     if (i >= 0 && i < a.n) {
-      const int slot = a.seq_map ? a.seq_map[i] : i;
-      const int64_t first = a.first ? a.first[i] : 0;
-      const int o = a.row_offsets[i];
       if (o < 0 || o > r) {
         bad = kErrRows;
       } else if (slot >= c.slots) {
         bad = kErrSlot;
       } else if (slot >= 0) {                 // (a negative slot is padding)
-        const int64_t t = first + (r - o);
-        const int len = c.lengths[slot];
-        if (t < 0 || t >= len || len / G > c.max_pages) {
-          bad = kErrLength;
-        } else {
-          const int b = int(t / G), in = int(t % G);
-          if (b < len / G) {
-            const int page = c.block_table[int64_t(slot) * c.bt_s_slot + b];
-            if (page < 0 || page >= c.pages) bad = kErrPage;
-            else at = RowAt{(int64_t(page) * H * G + in) * D, page};
-          } else {
-            at = RowAt{(int64_t(slot) * H * G + in) * D, -1};
-          }
-        }
+        const int64_t t = int64_t(first) + (r - o);
+        const bool fits = t >= 0 && t <= 0x7fffffff;
+        const int b = fits ? int(t) / G : 0, in = fits ? int(t) - b * G : 0;
+        const int page = fits && b < c.max_pages ? c.block_table[int64_t(slot) * c.bt_s_slot + b] : -1;
+        const int len = c.lengths[slot];      // on its way together with the page
+        if (!fits || t >= len || len / G > c.max_pages) bad = kErrLength;
+        else if (b >= len / G) at = RowAt{(int64_t(slot) * H * G + in) * D, -1};
+        else if (page < 0 || page >= c.pages) bad = kErrPage;
+        else at = RowAt{(int64_t(page) * H * G + in) * D, page};
       }
     }
-    if (bad) dev::flag(err, bad);
-    s_row[threadIdx.x] = at;
+    if (lane < count) {
+      if (bad) dev::flag(err, bad);
+      s_row[lane] = at;
+    }
   }
   __syncthreads();
   const int per = D / 8, vecs = H * per;
@@ -138,6 +153,7 @@ extern "C" int kitty_kv8_read(const KittyKv8ReadArgs* a, void* stream) {
   const int rc = check_cache(&a->cache, what);
   if (rc != KITTY_OK) return rc;
   if (a->n < 0 || a->rows < 0) return fail(KITTY_ERR_INVALID_ARGUMENT, what, "negative size");
+  if (a->n > 0x7fffff00) return fail(KITTY_ERR_UNSUPPORTED, what, "too many entries");     // n + 32 is an int
   if (a->n == 0 || a->rows == 0) return KITTY_OK;
   if (!a->key || !a->value || !a->row_offsets)
     return fail(KITTY_ERR_INVALID_ARGUMENT, what, "NULL key, value or row_offsets");
