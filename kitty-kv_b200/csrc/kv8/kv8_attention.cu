@@ -59,6 +59,7 @@ struct alignas(16) Note {
 
 struct Plan {
   int passes, pass_heads;              // query heads of a KV head in passes of pass_heads
+  uint32_t per_page;                   // 2^31 / (page_size / 32), rounded up: see blocks_of
   int warps;                           // of the whole grid
   float* part_ml;                      // [2 warps][pass_heads][2]  reference, sum
   float* part_o;                       // [2 warps][pass_heads][D]
@@ -129,24 +130,32 @@ struct Tiles {
   int paged, all, tail;                // tiles in pages, all tiles, tail tokens
   __device__ int units() const { return all ? all + kSetup : 0; }
 };
+// Whole pages of len >= 0 tokens: (len / 32) / k for pages of 32 k tokens, k <= 8, by a
+// product.  With c = ceil(2^31 / k) = (2^31 + e) / k, e < k, and n = len / 32 < 2^26,
+// n c / 2^31 is above n / k by n e / (k 2^31) < 1 / k, so it has the same whole part.
+__device__ __forceinline__ int blocks_of(const Plan& plan, int len) {
+  return int(__umulhi(uint32_t(len) >> 5 << 1, plan.per_page));
+}
 template <int kTile>
-__device__ __forceinline__ Tiles tiles_of(const KittyKv8Cache& c, int len) {
-  const int blocks = len / c.page_size, tail = len - blocks * c.page_size;
+__device__ __forceinline__ Tiles tiles_of(const KittyKv8Cache& c, const Plan& plan, int len) {
+  const int blocks = blocks_of(plan, len), tail = len - blocks * c.page_size;
   const int paged = blocks * (c.page_size / kTile);
   return Tiles{paged, paged + (tail + kTile / 2 - 1) / (kTile / 2), tail};
 }
 // Tokens of batch row b: 0 for padding (a negative slot), and where its slot or its length is
-// out of range.  (From L2: merge_kernel asks before it has waited, and the SM's L1 may hold
-// what was there before the last kernel on the stream.)
-__device__ __forceinline__ int tokens_of(const KittyKv8AttentionArgs& a, int b, uint32_t* err = nullptr) {
-  const int s = a.seq_map ? __ldcg(a.seq_map + b) : b;
+// out of range.  kL2: from L2, for merge_kernel, which asks before it has waited; the SM's L1 may
+// hold what was there before the last kernel on the stream.
+template <bool kL2 = false>
+__device__ __forceinline__ int tokens_of(const KittyKv8AttentionArgs& a, const Plan& plan, int b, uint32_t* err = nullptr) {
+  const auto get = [](const int32_t* p) { return kL2 ? __ldcg(p) : *p; };
+  const int s = a.seq_map ? get(a.seq_map + b) : b;
   if (s < 0) return 0;
   if (s >= a.cache.slots) {
     if (err) dev::flag(err, kErrSlot);
     return 0;
   }
-  const int len = __ldcg(a.cache.lengths + s);
-  if (len >= 0 && len / a.cache.page_size <= a.cache.max_pages) return len;
+  const int len = get(a.cache.lengths + s);
+  if (len >= 0 && blocks_of(plan, len) <= a.cache.max_pages) return len;
   if (err) dev::flag(err, kErrLength);
   return 0;
 }
@@ -158,13 +167,14 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
 }
 
 // Row b has `per_row` = H * passes segments of equal length.
-template <int kTile>
-__device__ __forceinline__ int units_of_row(const KittyKv8AttentionArgs& a, int b, uint32_t* err = nullptr) {
-  return b < a.batch ? tiles_of<kTile>(a.cache, tokens_of(a, b, err)).units() : 0;
+template <int kTile, bool kL2 = false>
+__device__ __forceinline__ int units_of_row(const KittyKv8AttentionArgs& a, const Plan& plan, int b,
+                                            uint32_t* err = nullptr) {
+  return b < a.batch ? tiles_of<kTile>(a.cache, plan, tokens_of<kL2>(a, plan, b, err)).units() : 0;
 }
 
 // The rows before a place, in units: thread t of a CTA has rows [t rows_each, (t + 1)
-// rows_each) (one warp at a time took 9 us for 256 rows, the CTA together takes 1).
+// rows_each).  For batches of more than kFew rows.
 struct Rows {
   int64_t before[kWarps * 32];         // units of the rows before each thread's
   int64_t total[kWarps];
@@ -179,7 +189,7 @@ __device__ __forceinline__ int64_t scan_rows(const KittyKv8AttentionArgs& a, con
   int64_t mine = 0;
 #pragma unroll 4
   for (int i = 0; i < rows_each; ++i) {
-    const int b = tid * rows_each + i, n = units_of_row<kTile>(a, b, blockIdx.x == 0 ? err : nullptr);
+    const int b = tid * rows_each + i, n = units_of_row<kTile>(a, plan, b, blockIdx.x == 0 ? err : nullptr);
     mine += n;
     if (blockIdx.x == 0 && n == 0 && b < a.batch)
       for (int k = 0; k < per_row; ++k) plan.notes[int64_t(b) * per_row + k].units = 0;
@@ -207,35 +217,79 @@ struct Place {
   int64_t begin;       // first unit of the segment found
   int b, seg;          // its batch row and its index among the row's segments
 };
-// By the whole warp, for at most 32 rows: `incl` gets the units up to and with row `lane`'s;
-// returns those of all rows.  (No barrier, and no second look at the lengths.)
-template <int kTile>
-__device__ __forceinline__ int64_t scan_few(const KittyKv8AttentionArgs& a, const Plan& plan, int per_row, int64_t& one,
-                                            int64_t& incl, uint32_t* err) {
-  const int lane = threadIdx.x & 31;
-  const bool flags = blockIdx.x == 0 && threadIdx.x < 32;
-  one = units_of_row<kTile>(a, lane, flags ? err : nullptr);
-  if (flags && one == 0 && lane < a.batch)
-    for (int k = 0; k < per_row; ++k) plan.notes[int64_t(lane) * per_row + k].units = 0;
-  incl = one;
-  for (int o = 1; o < a.batch; o <<= 1) {
+// The same for at most kFew rows, by every warp for itself: no barrier, no second look at the
+// lengths, and all its loads at once.  Lane t has rows [t each, (t + 1) each).  256 sequences of up
+// to 60 tokens take 14.0 us so, 15.3 by the whole CTA.
+constexpr int kFewEach = 8, kFew = 32 * kFewEach;
+struct FewRows {
+  int one[kFewEach];                   // units of each row's segments
+  int64_t mine, before;                // of this lane's rows, and of the rows before them
+};
+// Returns the units of all rows (one segment of each).  kEach: 1 for at most 32 rows (a
+// call of one sequence takes 10.7 us, with room for 8 rows a lane 11.4), or kFewEach.
+template <int kTile, int kEach>
+__device__ __forceinline__ int64_t scan_few(const KittyKv8AttentionArgs& a, const Plan& plan, int per_row, int each,
+                                            FewRows& r, uint32_t* err) {
+  const int lane = threadIdx.x & 31, b0 = lane * each;
+  int slot[kEach], len[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) slot[i] = i < each && b0 + i < a.batch ? (a.seq_map ? a.seq_map[b0 + i] : b0 + i) : -1;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) len[i] = slot[i] >= 0 && slot[i] < a.cache.slots ? a.cache.lengths[slot[i]] : 0;
+  r.mine = 0;
+  uint32_t bad = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    if (slot[i] >= a.cache.slots) bad |= kErrSlot;
+    if (len[i] < 0 || blocks_of(plan, len[i]) > a.cache.max_pages) {
+      len[i] = 0;
+      bad |= kErrLength;
+    }
+    r.one[i] = tiles_of<kTile>(a.cache, plan, len[i]).units();
+    r.mine += r.one[i];
+  }
+  if (blockIdx.x == 0 && threadIdx.x < 32) {
+    if (bad) dev::flag(err, bad);
+    for (int i = 0; i < kEach; ++i)
+      if (i < each && b0 + i < a.batch && r.one[i] == 0)
+        for (int k = 0; k < per_row; ++k) plan.notes[int64_t(b0 + i) * per_row + k].units = 0;
+  }
+  int64_t incl = r.mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
     const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
-  return __shfl_sync(0xffffffffu, incl, a.batch - 1);
+  r.before = incl - r.mine;
+  return __shfl_sync(0xffffffffu, incl, 31);
 }
-__device__ __forceinline__ Place locate_few(int per_row, int64_t one, int64_t incl, int64_t f) {
-  const int64_t start = (incl - one) * per_row;
-  const int b = __ffs(__ballot_sync(0xffffffffu, f >= start && f < incl * per_row)) - 1;
-  const int64_t at = __shfl_sync(0xffffffffu, start, b), len = __shfl_sync(0xffffffffu, one, b);
+template <int kEach>
+__device__ __forceinline__ Place locate_few(int per_row, int each, const FewRows& r, int64_t f) {
+  int64_t at = r.before * per_row;
+  const uint32_t hit = __ballot_sync(0xffffffffu, f >= at && f < at + r.mine * per_row);
+  int len = 1, b = (threadIdx.x & 31) * each;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {               // this lane's row that holds f, if it has it
+    const int64_t next = at + int64_t(r.one[i]) * per_row;
+    if (f >= next) {
+      at = next;
+      ++b;
+    } else if (f >= at) {
+      len = r.one[i];
+      break;
+    }
+  }
+  const int src = __ffs(hit) - 1;
+  at = __shfl_sync(0xffffffffu, at, src);
+  len = __shfl_sync(0xffffffffu, len, src);
   const int seg = int(quotient(f - at, len));
-  return Place{at + seg * len, b, seg};
+  return Place{at + int64_t(seg) * len, __shfl_sync(0xffffffffu, b, src), seg};
 }
 
 // By the whole warp: the segment that holds unit f (less than there are).
 template <int kTile>
-__device__ __forceinline__ Place locate(const KittyKv8AttentionArgs& a, int per_row, int rows_each, const Rows& s,
-                                        int64_t f) {
+__device__ __forceinline__ Place locate(const KittyKv8AttentionArgs& a, const Plan& plan, int per_row, int rows_each,
+                                        const Rows& s, int64_t f) {
   const int lane = threadIdx.x & 31;
   int found = 0;                       // threads whose rows begin at or before f
 #pragma unroll
@@ -244,7 +298,7 @@ __device__ __forceinline__ Place locate(const KittyKv8AttentionArgs& a, int per_
   Place r{0, b0, 0};
   int64_t before = s.before[found - 1] * per_row;
   for (int i = 0; i < rows_each; i += 32) {
-    const int one = i + lane < rows_each ? units_of_row<kTile>(a, b0 + i + lane) : 0;
+    const int one = i + lane < rows_each ? units_of_row<kTile>(a, plan, b0 + i + lane) : 0;
     int64_t incl = int64_t(one) * per_row;
     const int64_t mine = incl;
     if (rows_each > 1) {
@@ -309,22 +363,25 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
 
   // this warp's slice [f, f_end)
   __shared__ Rows s_rows;
-  const int rows_each = (a.batch + kWarps * 32 - 1) / (kWarps * 32);
-  int64_t row_one = 0, row_incl = 0;
-  const bool few = a.batch <= 32;
-  const int64_t total = (few ? scan_few<kTile>(a, plan, per_row, row_one, row_incl, err)
-                             : scan_rows<kTile>(a, plan, per_row, rows_each, s_rows, err)) * per_row;
+  const bool few = a.batch <= kFew;
+  const int row_threads = few ? 32 : kWarps * 32, rows_each = (a.batch + row_threads - 1) / row_threads;
+  FewRows few_rows;
+  const int64_t total = (rows_each == 1 && few ? scan_few<kTile, 1>(a, plan, per_row, 1, few_rows, err)
+                         : few ? scan_few<kTile, kFewEach>(a, plan, per_row, rows_each, few_rows, err)
+                               : scan_rows<kTile>(a, plan, per_row, rows_each, s_rows, err)) * per_row;
   const int64_t per_warp = quotient(total + plan.warps - 1, plan.warps);
   const int64_t f0 = warp * per_warp, f_end = min(total, f0 + per_warp);
   if (f0 >= f_end) return;
   if (warp == 0 && lane == 0) plan.notes[int64_t(a.batch) * per_row].units = per_warp;
-  const Place at = few ? locate_few(per_row, row_one, row_incl, f0) : locate<kTile>(a, per_row, rows_each, s_rows, f0);
+  const Place at = rows_each == 1 && few ? locate_few<1>(per_row, 1, few_rows, f0)
+                   : few ? locate_few<kFewEach>(per_row, rows_each, few_rows, f0)
+                         : locate<kTile>(a, plan, per_row, rows_each, s_rows, f0);
   int b = at.b, seg = at.seg;
   int64_t begin = at.begin;
 
   while (begin < f_end) {
-    const int len = tokens_of(a, b);
-    const Tiles tl = tiles_of<kTile>(c, len);
+    const int len = tokens_of(a, plan, b);
+    const Tiles tl = tiles_of<kTile>(c, plan, len);
     if (tl.all == 0) { ++b; continue; }             // (units are left, so a later row has some)
     const int slot = a.seq_map ? a.seq_map[b] : b;
     const int h = seg / plan.passes, q0 = (seg - h * plan.passes) * plan.pass_heads;
@@ -828,7 +885,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(KittyKv8AttentionA
   if (kTeam != 32 && a.batch <= 64) {                  // where the segment begins, while attention_kernel still runs
     int64_t before = 0, total = 0;
     for (int i = threadIdx.x & 31; i < a.batch; i += 32) {
-      const int64_t n = units_of_row<kTile>(a, i);
+      const int64_t n = units_of_row<kTile, true>(a, plan, i);
       total += n;
       if (i < b) before += n;
     }
@@ -838,7 +895,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(KittyKv8AttentionA
       before += __shfl_xor_sync(0xffffffffu, before, o);
     }
     per_warp = max(quotient(total * per_row + plan.warps - 1, plan.warps), int64_t(1));
-    note.units = units_of_row<kTile>(a, b);
+    note.units = units_of_row<kTile, true>(a, plan, b);
     note.begin = before * per_row + int64_t(seg) * note.units;
   }
   dev::wait_for_stream();                              // attention_kernel is done and its parts are visible
@@ -999,6 +1056,8 @@ int launch_heads(const KittyKv8AttentionArgs& a, uint32_t* err, cudaStream_t s, 
   const int g = a.num_q_heads / a.cache.num_heads;
   constexpr bool kTwo = kDim <= 128;
   Plan plan{};
+  const uint32_t k = uint32_t(a.cache.page_size) / 32;
+  plan.per_page = (0x80000000u + k - 1) / k;
   const int most = kTwo && g > 8 ? 16 : 8;
   plan.passes = (g + most - 1) / most;
   plan.pass_heads = (g + plan.passes - 1) / plan.passes;

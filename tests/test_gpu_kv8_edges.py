@@ -125,6 +125,27 @@ def test_batches_around_the_scan_sizes(batch):
     assert K.kv8_error_flags() == 0
 
 
+@pytest.mark.parametrize("batch", [64, 65, 255, 256, 257])
+def test_batches_around_the_scan_sizes_mapped_and_with_faults(batch):
+    """Slots in another order, some twice, some empty, padded, out of range or of a wrong length."""
+    g = torch.Generator().manual_seed(batch)
+    lens = torch.randint(0, 200, (90,), generator=g).tolist()
+    lens[7], lens[8], lens[9] = 1500, 0, 70
+    m = filled(lens, 2, 64, 96, E4M3, FP16, seed=batch)
+    rows = torch.randint(0, 90, (batch,), generator=g).tolist()
+    rows[3], rows[5], rows[-1], rows[batch // 2], rows[batch // 2 + 1] = 7, 8, 7, -3, 90
+    n = m.lens()
+    n[9], n[10] = -4, 2 ** 31 - 1
+    q = torch.randn(batch, 6, 64, generator=m.g).to(FP16).cuda()
+    got = K.paged_attention_kv8(q, n, *m.arrays(), seq_map=i32(rows))
+    none = torch.tensor([s < 0 or s in (8, 9, 10, 90) for s in rows])
+    assert not got[none.cuda()].any()
+    some = [i for i in range(batch) if not none[i]]
+    check_attention(m, 6, rows=[rows[i] for i in some], q=q[some], got=got[some])
+    flags = (1 << 3) | ((1 << 4) if 9 in rows or 10 in rows else 0)
+    assert K.kv8_error_flags() == flags
+
+
 def test_all_slots_empty():
     m = CacheModel(40, 2, 128, 64, E4M3, BF16, pages=1, table_width=1, seed=6, fill=float("nan"))
     for b in (1, 40):
