@@ -11,7 +11,8 @@
 //
 // A block of one head (G x D values) is read once into registers where it fits, its
 // largest magnitude taken with packed 16-bit maxima (exact), and the codes stored from
-// registers: 2 bytes read and 1 written a value, the floor of this operation.
+// registers: 2 bytes read and 1 written a value, the floor of this operation.  Of small
+// blocks a CTA takes several heads, so that its threads have as much to do.
 #include "kv8_common.cuh"
 
 namespace kitty8 {
@@ -140,6 +141,57 @@ __device__ __forceinline__ void quantise_block(const KittyKv8Cache& c, int slot,
   }
 }
 
+// The same for a block's heads h .. h + heads - 1 (at most 2^shift), 2^-shift of the CTA's warps
+// for each, whose registers hold it.  kShift: the shift, known when compiled (75K ragged rows of
+// 8 heads of 128 in 32-token pages: 75 us, 85 otherwise), or -1.
+template <bool kBf16, int kCode, int kPer, int kShift>
+__device__ __forceinline__ void quantise_heads(const KittyKv8Cache& c, int slot, int block, int h, int heads, int shift_,
+                                               const Rows (&src)[2], const int64_t (&s_head)[2],
+                                               uint32_t (*s_top)[kThreads / 32], uint32_t* err) {
+  constexpr float kQ = kCode == KITTY_KV8_E4M3 ? 448.f : 127.f;
+  const int G = c.page_size, D = c.head_dim, vecs = G * vecs_of_row<kPer>(D);
+  const int shift = kShift < 0 ? shift_ : kShift, threads = kThreads >> shift, hh = threadIdx.x / threads, tid = threadIdx.x - hh * threads;
+  uint4 held[2][kHeld];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const Rows r{src[x].tail + int64_t(hh) * G * D, src[x].fresh + hh * s_head[x], src[x].s_row, src[x].have};
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int v = tid + i * threads;
+      held[x][i] = hh < heads && v < vecs ? load_vec<kPer>(r, D, v) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  const int page = page_of(c, slot, block, err);
+  if (page < 0) return;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    uint32_t top = 0u;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) top = top_of<kBf16>(held[x][i], top);
+    top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));     // (as integers NaN is above infinity)
+    if ((threadIdx.x & 31) == 0) s_top[x][threadIdx.x >> 5] = top;
+  }
+  __syncthreads();
+  if (hh >= heads) return;
+  const int64_t at = int64_t(page) * c.num_heads + h + hh;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < threads / 32; ++i) m = max(m, s_top[x][hh * (threads / 32) + i]);
+    const float a = dev::to_f2<kBf16>(m).x;
+    const float top_f = a < 0x1p-100f ? 0x1p-100f : a;
+    const float r = __frcp_rn(top_f) * kQ;
+    if (tid == 0) (x ? c.value_scale : c.key_scale)[at] = top_f * (1.f / kQ);
+    uint2* codes = reinterpret_cast<uint2*>(static_cast<uint8_t*>(x ? c.value_codes : c.key_codes) + at * G * D);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int v = tid + i * threads;
+      if (v < vecs) codes[v] = encode_vec<kBf16, kCode>(held[x][i], r);
+    }
+  }
+}
+
 // Entry i's slot, its rows [o, o + len) and the tokens it has; false for padding (a negative
 // slot), and (flagged) if any of them is out of range, or the slot is an earlier entry's.
 __device__ __forceinline__ bool entry_of(const KittyKv8WriteArgs& a, int i, bool first_cta, uint32_t* err, int& slot,
@@ -166,15 +218,18 @@ __device__ __forceinline__ const uint16_t* row_of(const void* base, int64_t row,
   return static_cast<const uint16_t*>(base) + row * s_row + h * s_head;
 }
 
-// Ragged rows.  CTAs run over the heads first: those that are resident together read whole
+// Ragged rows; each CTA 2^kShift heads (-1: 2^shift).  CTAs run over the heads first: those that are resident together read whole
 // rows of the tokens, and not one head's slice of many.
-template <bool kBf16, int kCode, int kPer>
-__global__ void __launch_bounds__(kThreads, kMinCtas) write_kernel(KittyKv8WriteArgs a, uint32_t* err) {
+template <bool kBf16, int kCode, int kPer, int kShift>
+__global__ void __launch_bounds__(kThreads, kMinCtas) write_kernel(KittyKv8WriteArgs a, int shift_, uint32_t* err) {
   __shared__ uint32_t s_top[2][kThreads / 32];
   dev::wait_for_stream();
   const KittyKv8Cache& c = a.cache;
   const int G = c.page_size, D = c.head_dim;
-  const int item = blockIdx.x / c.num_heads, h = blockIdx.x - item * c.num_heads;
+  const int shift = kShift < 0 ? shift_ : kShift, groups = (c.num_heads + (1 << shift) - 1) >> shift;
+  const int item = blockIdx.x / groups, h = (blockIdx.x - item * groups) << shift;
+  const int heads = min(1 << shift, c.num_heads - h);
+  [[maybe_unused]] const int64_t s_head[2] = {a.k_s_head, a.v_s_head};
   int slot, o, len, cached;
   if (item < a.n) {
     if (!entry_of(a, item, h == 0, err, slot, o, len, cached)) return;
@@ -189,15 +244,19 @@ __global__ void __launch_bounds__(kThreads, kMinCtas) write_kernel(KittyKv8Write
     if (whole) {
       const Rows src[2] = {{tail_k, row_of(a.key, o, a.k_s_row, h, a.k_s_head), a.k_s_row, have},
                            {tail_v, row_of(a.value, o, a.v_s_row, h, a.v_s_head), a.v_s_row, have}};
-      quantise_block<kBf16, kCode, kPer>(c, slot, block, h, src, s_top, err);
+      if constexpr (kShift != 0)
+        quantise_heads<kBf16, kCode, kPer, kShift>(c, slot, block, h, heads, shift, src, s_head, s_top, err);
+      else
+        quantise_block<kBf16, kCode, kPer>(c, slot, block, h, src, s_top, err);
       __syncthreads();   // every thread has read the tail rows of the block
     }
-    for (int u = threadIdx.x; u < 2 * left * per; u += kThreads) {
-      const int x = u >= left * per, v = u - x * left * per, t = v / per, d = v - t * per;
-      const uint16_t* src = x ? row_of(a.value, o + len - left + t, a.v_s_row, h, a.v_s_head)
-                              : row_of(a.key, o + len - left + t, a.k_s_row, h, a.k_s_head);
-      reinterpret_cast<uint4*>((x ? tail_v : tail_k) + (to + t) * D)[d] = reinterpret_cast<const uint4*>(src)[d];
-    }
+    for (int hh = 0; hh < heads; ++hh)
+      for (int u = threadIdx.x; u < 2 * left * per; u += kThreads) {
+        const int x = u >= left * per, v = u - x * left * per, t = v / per, d = v - t * per;
+        const uint16_t* src = x ? row_of(a.value, o + len - left + t, a.v_s_row, h + hh, a.v_s_head)
+                                : row_of(a.key, o + len - left + t, a.k_s_row, h + hh, a.k_s_head);
+        reinterpret_cast<uint4*>((x ? tail_v : tail_k) + (hh * G + to + t) * D)[d] = reinterpret_cast<const uint4*>(src)[d];
+      }
   } else {
     const int64_t last = int64_t(item - a.n) * G + G - 1;              // < rows by the grid's size
     const int i = dev::count_le(a.row_offsets, a.n + 1, int(last)) - 1;
@@ -210,7 +269,10 @@ __global__ void __launch_bounds__(kThreads, kMinCtas) write_kernel(KittyKv8Write
     if (first < 0 || first + G > len) return;
     const Rows src[2] = {{nullptr, row_of(a.key, o + first, a.k_s_row, h, a.k_s_head), a.k_s_row, 0},
                          {nullptr, row_of(a.value, o + first, a.v_s_row, h, a.v_s_head), a.v_s_row, 0}};
-    quantise_block<kBf16, kCode, kPer>(c, slot, block, h, src, s_top, err);
+    if constexpr (kShift != 0)
+      quantise_heads<kBf16, kCode, kPer, kShift>(c, slot, block, h, heads, shift, src, s_head, s_top, err);
+    else
+      quantise_block<kBf16, kCode, kPer>(c, slot, block, h, src, s_top, err);
   }
 }
 
@@ -270,13 +332,29 @@ __global__ void __launch_bounds__(kThreads, kMinCtas) write_step_kernel(KittyKv8
 
 template <bool kBf16, int kCode, int kPer>
 int launch(const KittyKv8WriteArgs& a, uint32_t* err, cudaStream_t s) {
-  const int64_t H = a.cache.num_heads;
-  const int64_t ctas = a.row_offsets ? (int64_t(a.n) + a.rows / a.cache.page_size) * H
-                                     : (int64_t(a.n) + kStepEntries - 1) / kStepEntries * H + a.n;
-  if (ctas > 0x7fffffff) return fail(KITTY_ERR_UNSUPPORTED, "kv8_write", "too many rows times heads for one launch");
-  const dim3 grid{unsigned(ctas)};
-  return a.row_offsets ? launch_dependent("kv8_write", write_kernel<kBf16, kCode, kPer>, grid, kThreads, 0, s, a, err)
-                       : launch_dependent("kv8_write", write_step_kernel<kBf16, kCode, kPer>, grid, kThreads, 0, s, a, err);
+  const int64_t H = a.cache.num_heads, items = int64_t(a.n) + a.rows / a.cache.page_size;
+  const int64_t steps = (int64_t(a.n) + kStepEntries - 1) / kStepEntries * H + a.n;
+  // Heads of a CTA: as many as its registers hold, unless fewer than the card's CTAs are left
+  // to share the work.  75K ragged rows of 8 heads of 64 in 32-token pages take 40.5 us, with one
+  // head each 115; 300 rows 4.1, with four heads each 5.4.
+  const int vecs = a.cache.page_size * a.cache.head_dim / 8;
+  int shift = 0;
+  const auto ctas = [&] { return items * ((H + (1 << shift) - 1) >> shift); };
+  while (shift < 3 && (vecs << (shift + 1)) <= kHeld * kThreads && (1 << shift) < H &&
+         ctas() > int64_t(sm_count()) * kMinCtas)
+    ++shift;
+  const int64_t grid = a.row_offsets ? ctas() : steps;
+  if (grid > 0x7fffffff) return fail(KITTY_ERR_UNSUPPORTED, "kv8_write", "too many rows times heads for one launch");
+  const auto go = [&](auto kernel, auto... args) {
+    return launch_dependent("kv8_write", kernel, dim3(unsigned(grid)), kThreads, 0, s, a, args..., err);
+  };
+  if (!a.row_offsets) return go(write_step_kernel<kBf16, kCode, kPer>);
+  if (shift == 0) return go(write_kernel<kBf16, kCode, kPer, 0>, 0);
+  if constexpr (kPer == 0) return go(write_kernel<kBf16, kCode, 0, -1>, shift);
+  if constexpr (kPer == 8)
+    if (shift == 2) return go(write_kernel<kBf16, kCode, 8, 2>, 2);
+  if constexpr (kPer == 8 || kPer == 16) return go(write_kernel<kBf16, kCode, kPer, 1>, 1);
+  return fail(KITTY_ERR_UNSUPPORTED, "kv8_write", "no kernel");     // (the smallest block of 256 channels fills the registers)
 }
 
 template <bool kBf16, int kCode>

@@ -146,6 +146,43 @@ def test_batches_around_the_scan_sizes_mapped_and_with_faults(batch):
     assert K.kv8_error_flags() == flags
 
 
+@pytest.mark.parametrize("code,dtype", [(E4M3, FP16), (INT8, BF16)])
+@pytest.mark.parametrize("heads,dim,page,rows", [(8, 64, 32, 6000), (5, 64, 32, 6000), (3, 64, 64, 13000), (2, 64, 32, 10000),
+                                                 (8, 128, 32, 4000), (3, 128, 32, 7000), (16, 16, 32, 6000),
+                                                 (7, 80, 32, 4000), (9, 48, 64, 5000), (1, 64, 32, 20000)])
+def test_large_writes_of_small_blocks(code, dtype, heads, dim, page, rows):
+    """Enough rows that a CTA quantises several heads: rows of a fused projection, slots that have
+    begun a block, NaN and infinities in some heads' blocks, and pages that are none."""
+    n = 20
+    m = CacheModel(n, heads, dim, page, code, dtype, pages=rows // page + 3 * n, table_width=rows // page, seed=dim + rows)
+    write(m, range(n), [i * 7 % page for i in range(n)])
+    g = torch.Generator().manual_seed(rows)
+    counts = torch.distributions.Multinomial(rows, torch.rand(n, generator=g)).sample().int().tolist()
+    counts[4] = 0
+    both = torch.cat([m.new_rows(sum(counts)), m.new_rows(sum(counts))], 1)
+    both[40, 0, 3], both[900, heads - 1, 2], both[1700, heads, 5] = float("nan"), float("inf"), float("nan")
+    both[2000:2200] = 0
+    before, offsets = m.lens(), [0]
+    for s, c in enumerate(counts):
+        m.append(s, *both[offsets[-1]:offsets[-1] + c].split(heads, 1))
+        offsets.append(offsets[-1] + c)
+    table = m.table.clone()
+    lost = [s for s in range(n) if m.lengths[s] // page > 3][:2]
+    for s in lost:
+        table[s, 2] = 10 ** 6 if s == lost[0] else -1
+    key, value = both.cuda().split(heads, 1)
+    tails = m.tail_k.clone(), m.tail_v.clone()               # a write takes the rows of a begun block from them
+    K.write_kv8(key, value, before, *m.arrays(table), row_offsets=i32(offsets))
+    assert K.kv8_error_flags() == (1 << 1 if lost else 0)
+    spare = m.table[lost, 2].long().cuda()
+    for t in (m.key_codes, m.value_codes):
+        assert not t.view(torch.uint8)[spare].any()          # nothing went to the pages that were not named
+    m.tail_k.copy_(tails[0]), m.tail_v.copy_(tails[1])
+    K.write_kv8(key, value, before, *m.arrays(), row_offsets=i32(offsets))
+    assert K.kv8_error_flags() == 0
+    check_cache(m)
+
+
 def test_all_slots_empty():
     m = CacheModel(40, 2, 128, 64, E4M3, BF16, pages=1, table_width=1, seed=6, fill=float("nan"))
     for b in (1, 40):
