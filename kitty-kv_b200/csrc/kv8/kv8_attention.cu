@@ -24,9 +24,11 @@
 // 8-bit codes become fp16 exactly (e4m3 by conversion, int8 by the exponent trick), so
 // the products are exact and the sums float32.  q is fp16; a bf16 q is scaled by a power
 // of two per head that puts its largest element near the top of fp16's range, which
-// keeps elements down to 2^-29 of it exact.  Weights are rounded to fp16, off by at most
-// 2^-11 of themselves or 2^-31 of the one at the reference; for fp16 outputs, whose own
-// rounding is as small, they are split in two parts (16-bit tails: two parts of the type).
+// keeps elements down to 2^-29 of it exact.  A weight is the sum of fp16 parts, two of 11 bits:
+// off by at most 2^-22 of itself or 2^-31 of the one at the reference (bf16 tails: three
+// parts of 8 bits).  With one part, 2^-12, the bf16 outputs over 32 x 32K tokens are 6e-4
+// (root mean square) from those of float32 weights, so 6e-5; that second part costs 3 % there
+// (337 against 326 us), 15 % with 16 query heads on a KV head (254 against 222).
 //
 // All segments' tiles (kTile tokens of a page, half as many of a tail: about the same
 // bytes) are laid end to end, each segment's behind kSetup units that stand for what a
@@ -347,7 +349,8 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
   constexpr int kVH = kDim == 256 ? 2 : 1;          // 128-channel halves of a value row
   constexpr int kVW = kDim == 64 ? 2 : 4;           // words of codes a lane loads of a value row's half
   constexpr int kOT = kDim / 16;                    // output tiles
-  constexpr int kParts = kBf16 ? 1 : 2;             // fp16 parts of a weight in the paged tiles
+  constexpr int kParts = 2;                         // fp16 parts of a weight in the paged tiles
+  constexpr int kTailParts = kBf16 ? 3 : 2;         // parts of the tails' type in the tails
   constexpr int kTailRows = kTailTile / 8;          // token rows of a score tile that a tail tile fills
   __shared__ float4 s_o[kNT * kOT][kWarps][32];     // outputs of the CTA's warps where they share a segment
   __shared__ float s_m[kWarps][kNT * 8], s_l[kWarps][kNT * 8];
@@ -664,12 +667,10 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const uint32_t hi = dev::from_f2<false>(s[nt][mt][2 * r], s[nt][mt][2 * r + 1]);
+            const float2 back = dev::to_f2<false>(hi);
             wb[nt][mt][0][r] = transpose8x8(hi);
-            if constexpr (kParts == 2) {
-              const float2 back = dev::to_f2<false>(hi);
-              wb[nt][mt][kParts - 1][r] =
-                  transpose8x8(dev::from_f2<false>(s[nt][mt][2 * r] - back.x, s[nt][mt][2 * r + 1] - back.y));
-            }
+            wb[nt][mt][1][r] =
+                transpose8x8(dev::from_f2<false>(s[nt][mt][2 * r] - back.x, s[nt][mt][2 * r + 1] - back.y));
             l[nt][0] += s[nt][mt][2 * r];
             l[nt][1] += s[nt][mt][2 * r + 1];
           }
@@ -731,16 +732,20 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
           }
         }
       if (t + 1 < t1) load_tail_keys(t + 1);
-      uint32_t wb[kNT][2][2];                     // two parts of the tails' type
+      uint32_t wb[kNT][kTailParts][2];
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) {
         weigh(s[nt], nt, fac16, fac16, [&](int, int row) { return row < kTailRows && tok + 8 * row < tl.tail; });
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const uint32_t hi = dev::from_f2<kBf16>(s[nt][0][2 * r], s[nt][0][2 * r + 1]);
-          const float2 back = dev::to_f2<kBf16>(hi);
-          wb[nt][0][r] = transpose8x8(hi);
-          wb[nt][1][r] = transpose8x8(dev::from_f2<kBf16>(s[nt][0][2 * r] - back.x, s[nt][0][2 * r + 1] - back.y));
+          float2 left = make_float2(s[nt][0][2 * r], s[nt][0][2 * r + 1]);
+#pragma unroll
+          for (int p = 0; p < kTailParts; ++p) {  // each takes what the ones before leave
+            const uint32_t part = dev::from_f2<kBf16>(left.x, left.y);
+            const float2 back = dev::to_f2<kBf16>(part);
+            wb[nt][p][r] = transpose8x8(part);
+            left = make_float2(left.x - back.x, left.y - back.y);
+          }
         }
         l[nt][0] += s[nt][0][0] + s[nt][0][2];
         l[nt][1] += s[nt][0][1] + s[nt][0][3];
@@ -757,8 +762,8 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
           const uint32_t a2 = prmt(w2, w3, 0x5410), a3 = prmt(w2, w3, 0x7632);
 #pragma unroll
           for (int nt = 0; nt < kNT; ++nt) {
-            mma<kBf16>(o[nt][i], a0, a1, a2, a3, wb[nt][0][0], wb[nt][0][1]);
-            mma<kBf16>(o[nt][i], a0, a1, a2, a3, wb[nt][1][0], wb[nt][1][1]);
+#pragma unroll
+            for (int p = 0; p < kTailParts; ++p) mma<kBf16>(o[nt][i], a0, a1, a2, a3, wb[nt][p][0], wb[nt][p][1]);
           }
         }
       if (t + 1 < t1) load_tail_values(t + 1);

@@ -71,7 +71,8 @@ def paged_attention_kv8(q: torch.Tensor, lengths: torch.Tensor, block_table: tor
 
     Row b attends to all ``lengths[slot]`` tokens of slot ``seq_map[b]`` ((B,) int32;
     without it b), query head qh to KV head ``qh // (Hq // H)``; softmax and sums in
-    float32, scores scaled by ``sm_scale`` (default 1 / sqrt(D)).  An empty slot gives
+    float32, scores scaled by ``sm_scale`` (default 1 / sqrt(D)).  The weights that multiply the
+    values are off by at most 2^-22 of themselves, or 2^-31 of the largest.  An empty slot gives
     zeros, and so does a negative one (a padded batch).  The same call gives the same bits;
     which tokens are summed together depends on the whole batch's lengths.  Two launches; the scratch they share is allocated for each call, so calls on
     several streams or in several graphs do not meet.

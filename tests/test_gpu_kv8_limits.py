@@ -1,0 +1,51 @@
+"""GPU tests of the 8-bit cache's attention at the limits of its inputs: pages that are none
+beside pages of NaN, NaN in one tile of many, the largest values, and how exactly the weights
+are held."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from kitty import kernels as K
+from kv8_model import CacheModel, attention
+from test_gpu_kv8 import BF16, E4M3, FP16, INT8, filled, i32
+
+pytestmark = pytest.mark.gpu
+
+
+def bound(out, absum, mass, dtype):
+    """Bound of |kernel - exact| with weights held in 22 bits or more: a score is off by at most 64
+    roundings of 2^-23 of its sum of magnitudes, a weight by that, the exponential's 2^-20 and the
+    2^-22 that two fp16 parts leave of it; that counts in numerator and denominator; the output is
+    rounded once, half a step or half the smallest subnormal."""
+    w = 64 * 2.0 ** -23 * mass + 2.0 ** -20 + 2.0 ** -22
+    return torch.finfo(dtype).eps / 2 * out.abs() + 2 * w * absum * (1 + torch.finfo(dtype).eps) + 2.0 ** -25
+
+
+def check(m, q, got, slot, i, keep=None):
+    k, v = m.truth(slot)
+    if keep is not None:
+        k, v = k[:, keep], v[:, keep]
+    want, absum, mass = attention(q[i].cpu(), k, v)
+    err = (got[i].cpu().double() - want).abs()
+    assert (err <= bound(want, absum, mass, m.dtype)).all(), f"row {i}: {(err / bound(want, absum, mass, m.dtype)).max():.2f}"
+
+
+@pytest.mark.parametrize("code", [E4M3, INT8])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("heads,group,dim", [(2, 4, 128), (1, 16, 128), (2, 8, 64), (1, 3, 256), (1, 5, 80)])
+def test_weights_are_held_in_22_bits(code, dtype, heads, group, dim):
+    """Values of both signs nearly cancel, small queries make the weights alike: what is left shows
+    how far the weights are off, in pages and in the tail."""
+    lens = [32, 31, 64, 40, 2000]
+    m = CacheModel(len(lens), heads, dim, 32, code, dtype, pages=100, table_width=64, seed=dim + group)
+    for s, n in enumerate(lens):
+        v = m.new_rows(n)
+        v[1::2] = -v[:n // 2 * 2:2]
+        m.append(s, m.new_rows(n, 0.1), v)
+    m.fill_arrays()
+    q = (0.05 * torch.randn(len(lens), heads * group, dim, generator=m.g)).to(dtype).cuda()
+    got = K.paged_attention_kv8(q, m.lens(), *m.arrays())
+    for i in range(len(lens)):
+        check(m, q, got, i, i)
