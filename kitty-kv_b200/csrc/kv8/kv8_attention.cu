@@ -675,7 +675,12 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
             l[nt][1] += s[nt][mt][2 * r + 1];
           }
       }
-      const float vmul = ok_now ? vs_now : 0.f;
+      float vmul = vs_now;
+      if (!ok_now) {                              // page 0 stood in for it: its codes may be NaN, which no weight of 0 takes away
+        vmul = 0.f;
+#pragma unroll
+        for (int i = 0; i < kMT * kVH * 4 * kVW; ++i) vr[i] = 0u;
+      }
 #pragma unroll
       for (int vh = 0; vh < kVH; ++vh)
 #pragma unroll

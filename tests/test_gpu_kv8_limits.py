@@ -32,6 +32,31 @@ def check(m, q, got, slot, i, keep=None):
     assert (err <= bound(want, absum, mass, m.dtype)).all(), f"row {i}: {(err / bound(want, absum, mass, m.dtype)).max():.2f}"
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("heads,dim", [(1, 64), (2, 128), (1, 256)])
+@pytest.mark.parametrize("lens", [[96, 200], [4000, 5000]])
+def test_a_missing_page_does_not_let_page_0_in(dtype, heads, dim, lens):
+    """Page 0 is another sequence's, and holds NaN codes and scales; a block whose table entry is no
+    page is left out and flagged, and the rest of its sequence comes out."""
+    m = CacheModel(3, heads, dim, 32, E4M3, dtype, pages=2 + sum(n // 32 for n in lens), table_width=200, seed=dim)
+    m.free.remove(0)
+    m.free.append(0)                                      # slot 2's block
+    bad = m.new_rows(32)
+    bad[5, :, 3], bad[6, :, 9] = float("nan"), float("inf")
+    m.append(2, bad, bad)
+    for s, n in enumerate(lens):
+        m.append(s, m.new_rows(n), m.new_rows(n))
+    m.fill_arrays()
+    q = torch.randn(3, 4 * heads, dim, generator=m.g).to(dtype).cuda()
+    table = m.table.clone()
+    table[0, 1], table[1, 0], table[1, 4] = -1, 10 ** 6, m.key_scale.shape[0]
+    got = K.paged_attention_kv8(q, m.lens(), *m.arrays(table))
+    assert K.kv8_error_flags() == 1 << 1
+    assert got[2].isnan().all()
+    check(m, q, got, 0, 0, [t for t in range(lens[0]) if t // 32 != 1])
+    check(m, q, got, 1, 1, [t for t in range(lens[1]) if t // 32 not in (0, 4)])
+
+
 @pytest.mark.parametrize("code", [E4M3, INT8])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("heads,group,dim", [(2, 4, 128), (1, 16, 128), (2, 8, 64), (1, 3, 256), (1, 5, 80)])
