@@ -124,7 +124,8 @@ int kitty_kv8_read(const KittyKv8ReadArgs* args, void* stream);
  * lengths[slot] tokens of slot seq_map[b] (NULL: b), KV head qh / (Hq / H); zeros for
  * an empty slot and for a negative one (padding).  q and out have the cache's 16-bit type; sums and softmax statistics
  * are float32; the weights that multiply the values are off by at most 2^-22 of
- * themselves, or 2^-31 of the largest.  The workspace (16-byte aligned) holds the partial results of
+ * themselves, or 2^-31 of the largest.  bf16 values may be as large as 2^128 / tokens
+ * (a float32 sum of weights of at most 1).  The workspace (16-byte aligned) holds the partial results of
  * sequences that several warps share; calls that overlap must not share one. */
 typedef struct KittyKv8AttentionArgs {
   KittyKv8Cache cache;

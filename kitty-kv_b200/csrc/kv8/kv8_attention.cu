@@ -351,6 +351,9 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
   constexpr int kOT = kDim / 16;                    // output tiles
   constexpr int kParts = 2;                         // fp16 parts of a weight in the paged tiles
   constexpr int kTailParts = kBf16 ? 3 : 2;         // parts of the tails' type in the tails
+  // Outputs and sums are held in this unit, so that the largest weight counts as 1: a bf16 value
+  // may be anything below 2^128, and 2^14 of it would pass float32.
+  constexpr float kUnit = kBf16 ? 0x1p-14f : 1.f;
   constexpr int kTailRows = kTailTile / 8;          // token rows of a score tile that a tail tile fills
   __shared__ float4 s_o[kNT * kOT][kWarps][32];     // outputs of the CTA's warps where they share a segment
   __shared__ float s_m[kWarps][kNT * 8], s_l[kWarps][kNT * 8];
@@ -675,7 +678,7 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
             l[nt][1] += s[nt][mt][2 * r + 1];
           }
       }
-      float vmul = vs_now;
+      float vmul = vs_now * kUnit;
       if (!ok_now) {                              // page 0 stood in for it: its codes may be NaN, which no weight of 0 takes away
         vmul = 0.f;
 #pragma unroll
@@ -743,7 +746,7 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
         weigh(s[nt], nt, fac16, fac16, [&](int, int row) { return row < kTailRows && tok + 8 * row < tl.tail; });
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          float2 left = make_float2(s[nt][0][2 * r], s[nt][0][2 * r + 1]);
+          float2 left = make_float2(s[nt][0][2 * r] * kUnit, s[nt][0][2 * r + 1] * kUnit);
 #pragma unroll
           for (int p = 0; p < kTailParts; ++p) {  // each takes what the ones before leave
             const uint32_t part = dev::from_f2<kBf16>(left.x, left.y);
@@ -782,6 +785,7 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
         l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 4);
         l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 8);
         l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 16);
+        l[nt][j] *= kUnit;
       }
     const bool all_here = t0 == 0 && t1 == tl.all;
     if (t0 == 0 && lane == 0) plan.notes[segment] = all_here ? Note{0, -1} : Note{here, end - here};

@@ -58,6 +58,25 @@ def test_a_missing_page_does_not_let_page_0_in(dtype, heads, dim, lens):
 
 
 @pytest.mark.parametrize("code", [E4M3, INT8])
+@pytest.mark.parametrize("lens", [[5, 32, 61], [300, 96, 40], [9000, 3, 64]])
+def test_the_largest_values(code, lens):
+    """bf16 values up to 2^128 / tokens: every partial sum of weights of at most one fits float32, so
+    the outputs are finite, and right."""
+    m = CacheModel(3, 1, 64, 32, code, BF16, pages=sum(lens) // 32 + 3, table_width=300, seed=sum(lens))
+    for s, n in enumerate(lens):
+        top = 2.0 ** 127 / n
+        v = (torch.rand(n, 1, 64, generator=m.g) * 2 - 1) * 0.99 * top
+        v[n // 2, 0, 0] = top * 0.99
+        m.append(s, (m.new_rows(n) * torch.linspace(0.2, 1, n)[:, None, None]).to(BF16), v.to(BF16))
+    m.fill_arrays()
+    q = torch.randn(3, 4, 64, generator=m.g).to(BF16).cuda()
+    got = K.paged_attention_kv8(q, m.lens(), *m.arrays())
+    assert torch.isfinite(got).all()
+    for i in range(3):
+        check(m, q, got, i, i)
+
+
+@pytest.mark.parametrize("code", [E4M3, INT8])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("heads,group,dim", [(2, 4, 128), (1, 16, 128), (2, 8, 64), (1, 3, 256), (1, 5, 80)])
 def test_weights_are_held_in_22_bits(code, dtype, heads, group, dim):
