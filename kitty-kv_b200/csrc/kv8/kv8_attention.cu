@@ -590,9 +590,10 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
           }
       };
       relative(false);
-      // A score far above the reference, none yet, or NaN; or a reference so far out that its
+      // A score far above the reference, or none yet; or a reference so far out that its
       // rounding (it is a rounded product) is more than the weights' range, where the products
-      // have to be rounded alike.
+      // have to be rounded alike.  (The maxima drop NaN, so a NaN score moves no reference: its
+      // weight is NaN, and with it the output.)
       if (far || !__all_sync(0xffffffffu, top <= kHead + kSlack)) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {

@@ -57,6 +57,25 @@ def test_a_missing_page_does_not_let_page_0_in(dtype, heads, dim, lens):
     check(m, q, got, 1, 1, [t for t in range(lens[1]) if t // 32 not in (0, 4)])
 
 
+@pytest.mark.parametrize("code,dtype", [(E4M3, BF16), (E4M3, FP16), (INT8, BF16)])
+@pytest.mark.parametrize("group", [4, 16])
+def test_nan_in_one_key_tile_or_tail_row(code, dtype, group):
+    """NaN scores reach the output of their own sequence and head group, and no other."""
+    lens = [3000, 3000, 3010, 1]
+    m = filled(lens, 2, 128, 64, code, dtype, seed=group)
+    table = m.table
+    m.key_scale[int(table[0, 20]), 1] = float("nan")       # one page in the middle, KV head 1
+    m.tail_k[2, 0, 1, 7] = float("nan")                  # the second of the tail's two rows, KV head 0
+    q = torch.randn(4, 2 * group, 128, generator=m.g).to(dtype).cuda()
+    got = K.paged_attention_kv8(q, m.lens(), *m.arrays())
+    bad = torch.zeros(4, 2 * group, 128, dtype=torch.bool)
+    bad[0, group:], bad[2, :group] = True, True
+    assert torch.equal(got.isnan().cpu(), bad)
+    for i in (1, 3):
+        check(m, q, got, i, i)
+    assert K.kv8_error_flags() == 0
+
+
 @pytest.mark.parametrize("code", [E4M3, INT8])
 @pytest.mark.parametrize("lens", [[5, 32, 61], [300, 96, 40], [9000, 3, 64]])
 def test_the_largest_values(code, lens):
