@@ -41,7 +41,9 @@ def write_kv8(key: torch.Tensor, value: torch.Tensor, lengths: torch.Tensor, blo
     slot ``seq_map[i]`` has ((n,) int32, distinct; without it i; negative: padding,
     skipped).  Blocks that fill are quantised into the pages that ``block_table`` holds for
     them, the rest stays in the tail.  ``lengths`` is not changed: add the new tokens
-    before the next call on this cache.  Rows behind the last offset are ignored.
+    before the next call on this cache (torch's indexing takes no negative slot; of single rows
+    ``lengths.index_add_(0, seq_map.clamp(min=0), (seq_map >= 0).to(torch.int32))`` is safe with
+    padding).  Rows behind the last offset are ignored.
     """
     _kv8.ops().write(key, value, lengths, block_table, key_codes, value_codes, key_scale, value_scale, tail_k, tail_v,
                      row_offsets, seq_map)
