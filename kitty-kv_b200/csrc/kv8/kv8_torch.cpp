@@ -15,7 +15,9 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <limits>
 
 #include "../../../include/kitty_kv8.h"
@@ -110,6 +112,40 @@ void* output_rows(Tensor& t, const Tensor& like, const char* name, int64_t& s0, 
                                                                      (s0 >= d && s1 >= (n - 1) * s0 + d)),
               name, " has rows that overlap");
   return t.data_ptr();
+}
+
+// The places of (rows, heads, D) 16-bit values, strides in elements (0 where there is one).
+struct Places {
+  const void* p;
+  int64_t n, h, d, s0, s1;
+  bool operator==(const Places& o) const { return p == o.p && n == o.n && h == o.h && s0 == o.s0 && s1 == o.s1; }
+};
+
+Places places(const Tensor& t, const void* p, int64_t s0, int64_t s1) {
+  return Places{p, t.size(0), t.size(1), t.size(2), t.size(0) > 1 ? s0 : 0, t.size(1) > 1 ? s1 : 0};
+}
+
+// Whether two of them, of equally many rows, share a value.  Exact where their row strides are
+// the same (the parts of fused rows lie between one another); otherwise whether their ranges meet.
+bool meet(const Places& a, const Places& b) {
+  if (a.n == 0 || a.h == 0 || b.h == 0) return false;
+  const int64_t off = (reinterpret_cast<intptr_t>(b.p) - reinterpret_cast<intptr_t>(a.p)) / 2;
+  const int64_t wide_a = (a.h - 1) * a.s1 + a.d, wide_b = (b.h - 1) * b.s1 + b.d, s = a.s0;
+  if (off >= (a.n - 1) * a.s0 + wide_a || -off >= (b.n - 1) * b.s0 + wide_b) return false;
+  if (a.s0 != b.s0) return true;
+  if (s > 0) {     // the rows of one between those of the other
+    const int64_t in = (off % s + s) % s;
+    if (in >= wide_a && in + wide_b <= s) return false;
+  }
+  for (int64_t i = 0; i < a.h; ++i)
+    for (int64_t j = 0; j < b.h; ++j) {
+      // head j of b against head i of a, k rows away: | e + k s | < d for a k of -(n - 1) .. n - 1
+      const int64_t e = off + j * b.s1 - i * a.s1;
+      const int64_t k = s > 0 ? std::max(-(a.n - 1), std::min(a.n - 1, -e / s)) : 0;
+      for (int64_t x = std::max(k - 1, -(a.n - 1)); x <= std::min(k + 1, a.n - 1); ++x)
+        if (std::abs(e + x * s) < a.d) return true;
+    }
+  return false;
 }
 
 const int32_t* index(Tensor& t, const char* name, int64_t n) {
@@ -217,10 +253,19 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
     wk = wk.contiguous();
   }
   pos = pos.contiguous();
+  const bool given = q_out.defined() || k_out.defined();
   a.q_out = output_rows(q_out, q, "q_out", a.qo_s_row, a.qo_s_head);
   a.k_out = output_rows(k_out, k, "k_out", a.ko_s_row, a.ko_s_head);
   a.q = input_rows(q, a.q_s_row, a.q_s_head);
   a.k = input_rows(k, a.k_s_row, a.k_s_head);
+  if (given) {     // warps take the heads of a token apart, and read ahead of what they store
+    const Places in[2] = {places(q, a.q, a.q_s_row, a.q_s_head), places(k, a.k, a.k_s_row, a.k_s_head)},
+                 out[2] = {places(q_out, a.q_out, a.qo_s_row, a.qo_s_head), places(k_out, a.k_out, a.ko_s_row, a.ko_s_head)};
+    for (int i = 0; i < 2; ++i)
+      TORCH_CHECK((out[i] == in[i] || !meet(out[i], in[i])) && !meet(out[i], in[1 - i]), i ? "k_out" : "q_out",
+                  " overlaps an input (it may be ", i ? "k" : "q", " itself, with the same strides)");
+    TORCH_CHECK(!meet(out[0], out[1]), "q_out and k_out overlap");
+  }
   a.q_weight = ptr(wq);
   a.k_weight = ptr(wk);
   a.positions = ptr(pos);
@@ -294,6 +339,9 @@ PyObject* read(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
                 "key_out and value_out must be (", rows, ", ", shape[1], ", ", shape[2], ") ", c.tail_k.scalar_type(),
                 ", contiguous");
   }
+  const int64_t row = shape[1] * shape[2];
+  TORCH_CHECK(!meet(Places{ptr(out[0]), rows, 1, row, row, 0}, Places{ptr(out[1]), rows, 1, row, row, 0}),
+              "key_out and value_out overlap");
   a.key = ptr(out[0]);
   a.value = ptr(out[1]);
   a.n = i32(n, "entries");
@@ -327,6 +375,8 @@ PyObject* attention(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
   a.seq_map = index(map, "seq_map", b);
   a.out = output_rows(out, q, "out", a.out_s_seq, a.out_s_head);
   a.q = input_rows(q, a.q_s_seq, a.q_s_head);
+  const Places from = places(q, a.q, a.q_s_seq, a.q_s_head), to = places(out, a.out, a.out_s_seq, a.out_s_head);
+  TORCH_CHECK(from == to || !meet(from, to), "out overlaps q (it may be q itself, with the same strides)");
   a.batch = i32(b, "B");
   a.num_q_heads = i32(hq, "Hq");
   const c10::cuda::CUDAGuard guard(call.device);

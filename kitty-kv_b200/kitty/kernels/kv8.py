@@ -59,7 +59,7 @@ def read_kv8(lengths: torch.Tensor, block_table: torch.Tensor, key_codes: torch.
     Output rows ``row_offsets[i]`` .. ``row_offsets[i + 1] - 1`` are the tokens of slot
     ``seq_map[i]`` (without it i) from ``first[i]`` (without it 0) on.  Rows behind the
     last offset, of a negative slot, and of tokens that the slot does not have are left as they were
-    (``key_out`` / ``value_out``: the caller's tensors, contiguous).
+    (``key_out`` / ``value_out``: the caller's tensors, contiguous, not overlapping).
     """
     return _kv8.ops().read(lengths, block_table, key_codes, value_codes, key_scale, value_scale, tail_k, tail_v,
                            row_offsets, rows, first, seq_map, key_out, value_out)
@@ -76,7 +76,8 @@ def paged_attention_kv8(q: torch.Tensor, lengths: torch.Tensor, block_table: tor
     float32, scores scaled by ``sm_scale`` (default 1 / sqrt(D)).  The weights that multiply the
     values are off by at most 2^-22 of themselves, or 2^-31 of the largest.  An empty slot gives
     zeros, and so does a negative one (a padded batch).  The same call gives the same bits;
-    which tokens are summed together depends on the whole batch's lengths.  Two launches; the scratch they share is allocated for each call, so calls on
+    which tokens are summed together depends on the whole batch's lengths.  ``out`` may be q
+    itself (same strides); any other overlap of the two is refused.  Two launches; the scratch they share is allocated for each call, so calls on
     several streams or in several graphs do not meet.
     """
     return _kv8.ops().attention(q, lengths, block_table, key_codes, value_codes, key_scale, value_scale, tail_k, tail_v,

@@ -47,7 +47,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
     q_weight / k_weight: (D,) of q's dtype or float32, both or neither; without them
     there is no norm, only the rotation.
     interleaved: rotate channels (2i, 2i + 1) together instead of (i, i + R / 2).
-    q_out / k_out: given tensors, also q and k themselves (same strides); q and k may be
-    strided views, as of one fused projection.  D and R are multiples of 16, D <= 256.
+    q_out / k_out: given tensors, also q and k themselves (same strides); any other overlap
+    with an input or one another is refused.  q and k may be strided views, as of one fused
+    projection.  D and R are multiples of 16, D <= 256.
     """
     return _kv8.ops().qk_norm_rope(q, k, positions, table, q_weight, k_weight, eps, interleaved, q_out, k_out)
