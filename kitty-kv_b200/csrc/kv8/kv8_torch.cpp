@@ -8,6 +8,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/AutogradState.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -50,12 +51,23 @@ struct Call {
   }
 };
 
-// These operators have no backward pass: an input that asks for one is refused.
-void no_grad(std::initializer_list<const Tensor*> inputs) {
-  if (!at::GradMode::is_enabled()) return;
-  for (const Tensor* t : inputs)
-    TORCH_CHECK(!t->defined() || !t->requires_grad(), "this operator has no backward pass: call it under "
+// These operators have no backward pass and no forward derivative: a tensor that asks for one is
+// refused, what is written included.
+void no_grad(std::initializer_list<const Tensor*> tensors) {
+  const bool backward = at::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  for (const Tensor* t : tensors) {
+    if (!t->defined()) continue;
+    TORCH_CHECK(!backward || !t->requires_grad(), "this operator has no backward pass: call it under "
                 "torch.no_grad() or on detached tensors");
+    TORCH_CHECK(!forward || !t->_fw_grad(0).defined(), "this operator has no forward derivative: call it on the "
+                "primal of a dual tensor");
+  }
+}
+
+// What autograd has saved of a tensor that was written is no longer what it was.
+void written(std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
 }
 
 int dtype_code(const Tensor& t, const char* what) {
@@ -198,6 +210,7 @@ CacheArrays fill_cache(Call& call, PyObject* const* o, KittyKv8Cache& c) {
   TORCH_CHECK(r.key_codes.is_contiguous() && r.value_codes.is_contiguous() && r.key_scale.is_contiguous() &&
               r.value_scale.is_contiguous() && r.tail_k.is_contiguous() && r.tail_v.is_contiguous() &&
               r.lengths.is_contiguous(), "pools, scales, tails and lengths must be contiguous");
+  no_grad({&r.key_codes, &r.value_codes, &r.key_scale, &r.value_scale, &r.tail_k, &r.tail_v});
   c.key_codes = ptr(r.key_codes);
   c.value_codes = ptr(r.value_codes);
   c.key_scale = static_cast<float*>(ptr(r.key_scale));
@@ -227,7 +240,7 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
   Tensor q = call.arg(o[0], "q"), k = call.arg(o[1], "k"), pos = call.arg(o[2], "positions"),
          table = call.arg(o[3], "table"), wq = call.arg(o[4], "q_weight", true), wk = call.arg(o[5], "k_weight", true),
          q_out = call.arg(o[8], "q_out", true), k_out = call.arg(o[9], "k_out", true);
-  no_grad({&q, &k, &wq, &wk, &table});
+  no_grad({&q, &k, &wq, &wk, &table, &q_out, &k_out});
   KittyQkNormRopeArgs a{};
   a.eps = float(PyFloat_AsDouble(o[6]));
   a.interleaved = PyObject_IsTrue(o[7]);
@@ -278,6 +291,7 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
   a.head_dim = i32(d, "D");
   a.rot = i32(table.size(1), "R");
   launch(call, kitty_qk_norm_rope, a, "kitty_qk_norm_rope");
+  written({&q_out, &k_out});
   PyObject* r = PyTuple_New(2);
   if (!r) return nullptr;
   PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(q_out));
@@ -311,6 +325,7 @@ PyObject* write(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
   a.n = i32(n, "entries");
   a.rows = i32(rows, "N");
   launch(call, kitty_kv8_write, a, "kitty_kv8_write");
+  written({&c.key_codes, &c.value_codes, &c.key_scale, &c.value_scale, &c.tail_k, &c.tail_v});
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -325,6 +340,7 @@ PyObject* read(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
   Tensor offsets = call.arg(o[8], "row_offsets"), first = call.arg(o[10], "first", true),
          map = call.arg(o[11], "seq_map", true);
   Tensor out[2] = {call.arg(o[12], "key_out", true), call.arg(o[13], "value_out", true)};
+  no_grad({&out[0], &out[1]});
   const int64_t rows = PyLong_AsLongLong(o[9]);
   if (PyErr_Occurred()) return nullptr;
   const int64_t n = offsets.numel() - 1;
@@ -347,6 +363,7 @@ PyObject* read(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
   a.n = i32(n, "entries");
   a.rows = i32(rows, "rows");
   launch(call, kitty_kv8_read, a, "kitty_kv8_read");
+  written({&out[0], &out[1]});
   PyObject* r = PyTuple_New(2);
   if (!r) return nullptr;
   PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(out[0]));
@@ -362,9 +379,9 @@ PyObject* attention(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
   Call call;
   KittyKv8AttentionArgs a{};
   Tensor q = call.arg(o[0], "q");
-  no_grad({&q});
   const CacheArrays c = fill_cache(call, o + 1, a.cache);
   Tensor map = call.arg(o[10], "seq_map", true), out = call.arg(o[11], "out", true);
+  no_grad({&q, &out});
   TORCH_CHECK(q.dim() == 3 && q.size(2) == a.cache.head_dim && q.scalar_type() == c.tail_k.scalar_type(),
               "q must be (B, Hq, ", a.cache.head_dim, ") ", c.tail_k.scalar_type());
   const int64_t b = q.size(0), hq = q.size(1);
@@ -385,6 +402,7 @@ PyObject* attention(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
   const c10::DataPtr scratch = c10::cuda::CUDACachingAllocator::get()->allocate(a.workspace_bytes);
   a.workspace = scratch.get();
   launch(call, kitty_kv8_attention, a, "kitty_kv8_attention");
+  written({&out});
   return THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
 }

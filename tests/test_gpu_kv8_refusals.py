@@ -82,3 +82,75 @@ def test_read_and_attention_outputs_that_overlap_are_refused():
     out = big[:2, 4:]
     assert K.paged_attention_kv8(big[:2, :4], m.lens(), *m.arrays(), out=out) is out and torch.equal(out, want)
     assert K.kv8_error_flags() == 0
+
+
+def grad_cases():
+    """(name, call of the tensors by name) of every operator; the tensors may be replaced."""
+    m = filled([70, 33], 1, 64, 32, E4M3, FP16, seed=2)
+    names = ("block_table", "key_codes", "value_codes", "key_scale", "value_scale", "tail_k", "tail_v")
+    t = dict(zip(names, (x.clone() for x in m.arrays())), lengths=m.lens(), q=torch.randn(2, 2, 64).half().cuda(),
+             k=torch.randn(2, 1, 64).half().cuda(), v=torch.randn(2, 1, 64).half().cuda(), wq=torch.ones(64).cuda(),
+             wk=torch.ones(64).cuda(), table=K.rope_table(4, 64, device="cuda"), q_out=torch.empty(2, 2, 64).half().cuda(),
+             k_out=torch.empty(2, 1, 64).half().cuda(), key_out=torch.empty(103, 1, 64).half().cuda(),
+             value_out=torch.empty(103, 1, 64).half().cuda(), off=i32([0, 70, 103]), pos=i32([0, 1]))
+
+    def cache(t):
+        return (t["lengths"], *(t[n] for n in names))
+
+    calls = {
+        "rope": (lambda t: K.qk_norm_rope(t["q"], t["k"], t["pos"], t["table"], t["wq"], t["wk"], q_out=t["q_out"], k_out=t["k_out"]),
+                 ("q", "k", "wq", "wk", "table", "q_out", "k_out"), ("q_out", "k_out")),
+        "write": (lambda t: K.write_kv8(t["k"], t["v"], *cache(t)), ("k", "v", "key_scale", "value_scale", "tail_k", "tail_v"),
+                  ("key_codes", "value_codes", "key_scale", "value_scale", "tail_k", "tail_v")),
+        "read": (lambda t: K.read_kv8(*cache(t), t["off"], 103, key_out=t["key_out"], value_out=t["value_out"]),
+                 ("key_scale", "value_scale", "tail_k", "tail_v", "key_out", "value_out"), ("key_out", "value_out")),
+        "attention": (lambda t: K.paged_attention_kv8(t["q"], *cache(t), out=t["q_out"]),
+                      ("q", "key_scale", "value_scale", "tail_k", "tail_v", "q_out"), ("q_out",))}
+    return t, calls
+
+
+@pytest.mark.parametrize("what", ["rope", "write", "read", "attention"])
+def test_tensors_that_ask_for_derivatives_are_refused(what):
+    import torch.autograd.forward_ad as fw
+    t, calls = grad_cases()
+    call, asks, written = calls[what]
+    before = {n: x.view(torch.uint8).clone() for n, x in t.items()}
+    for name in asks:
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            call({**t, name: t[name].detach().requires_grad_()})
+        with fw.dual_level():
+            dual = fw.make_dual(t[name], torch.ones_like(t[name]))
+            with pytest.raises(RuntimeError, match="no forward derivative"):
+                call({**t, name: dual})
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no forward derivative"):
+                call({**t, name: dual})
+    assert all(torch.equal(x.view(torch.uint8), before[n]) for n, x in t.items())
+    with torch.no_grad():                                  # as with torch's own operators, in place too
+        for name in asks:
+            call({**t, name: t[name].detach().requires_grad_()})
+
+
+@pytest.mark.parametrize("what", ["rope", "write", "read", "attention"])
+def test_what_is_written_counts_as_changed(what):
+    """A backward pass that saved what a call has since written raises; inference tensors are taken."""
+    t, calls = grad_cases()
+    call, _, written = calls[what]
+    for name in written:
+        if t[name].dtype == E4M3:
+            v = t[name]._version
+            call(t)
+            assert t[name]._version > v
+            continue
+        x = torch.ones_like(t[name], requires_grad=True)
+        y = (x * t[name]).sum()
+        call(t)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    reads = {n: x._version for n, x in t.items() if n not in written}
+    call(t)
+    assert all(t[n]._version == v for n, v in reads.items())
+    with torch.inference_mode():
+        own = {n: x.clone() for n, x in t.items()}
+        call(own)
+    call(own)
+    assert K.kv8_error_flags() == 0
