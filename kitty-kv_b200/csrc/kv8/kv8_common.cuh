@@ -47,7 +47,9 @@ int launch_dependent(const char* what, void (*kernel)(Params...), dim3 grid, int
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
-  return e == cudaSuccess ? KITTY_OK : fail(KITTY_ERR_CUDA, what, cudaGetErrorString(e));
+  if (e == cudaSuccess) return KITTY_OK;
+  cudaGetLastError();                  // reported here, and not to whoever asks next
+  return fail(KITTY_ERR_CUDA, what, cudaGetErrorString(e));
 }
 
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
