@@ -45,7 +45,8 @@ __global__ void __launch_bounds__(kThreads) read_kernel(KittyKv8ReadArgs a, uint
     if (__shfl_sync(0xffffffffu, offset, lo) <= r) ++lo;          // (31 of them, or 32)
     const int from = max(lo - 1, 0);
     int i = at0 + lo - 1, o = __shfl_sync(0xffffffffu, offset, from), slot = __shfl_sync(0xffffffffu, window_slot, from),
-        first = __shfl_sync(0xffffffffu, window_first, from);
+        first = __shfl_sync(0xffffffffu, window_first, from), end = __shfl_sync(0xffffffffu, offset, min(from + 1, 31));
+    if (from == 31) end = i < a.n ? a.row_offsets[i + 1] : 0;
     if (lo == 32 && at0 + 32 <= a.n) {   // the row is behind the window: many entries of no or few rows
       int hi = a.n + 1;
       lo = at0 + 32;
@@ -57,6 +58,7 @@ __global__ void __launch_bounds__(kThreads) read_kernel(KittyKv8ReadArgs a, uint
       i = lo - 1;
       o = a.row_offsets[i];
       if (i < a.n) {
+        end = a.row_offsets[i + 1];
         slot = a.seq_map ? a.seq_map[i] : i;
         first = a.first ? a.first[i] : 0;
       }
@@ -64,7 +66,7 @@ __global__ void __launch_bounds__(kThreads) read_kernel(KittyKv8ReadArgs a, uint
     RowAt at{0, -2};
     uint32_t bad = 0;
     if (i >= 0 && i < a.n) {
-      if (o < 0 || o > r) {
+      if (o < 0 || o > r || end <= r) {       // (offsets that decrease)
         bad = kErrRows;
       } else if (slot >= c.slots) {
         bad = kErrSlot;
@@ -84,6 +86,13 @@ __global__ void __launch_bounds__(kThreads) read_kernel(KittyKv8ReadArgs a, uint
       if (bad) dev::flag(err, bad);
       s_row[lane] = at;
     }
+  } else {                               // the other warps look all offsets over
+    uint32_t bad = 0;
+    for (int64_t i = int64_t(blockIdx.x) * (kThreads - 32) + threadIdx.x - 32; i < a.n; i += int64_t(gridDim.x) * (kThreads - 32)) {
+      const int o = a.row_offsets[i], end = a.row_offsets[i + 1];
+      if (o < 0 || end < o || end > a.rows) bad = kErrRows;
+    }
+    if (bad) dev::flag(err, bad);
   }
   __syncthreads();
   const int per = D / 8, vecs = H * per;
