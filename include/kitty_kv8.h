@@ -28,7 +28,8 @@
  * Errors that only device data shows skip what they concern, never touch memory out
  * of bounds, and set a sticky bit (kitty_kv8_error_flags):
  *   bit 1  a page number outside the pool, or a block past the block table's row
- *   bit 2  row offsets that decrease, are negative or pass the rows of the call
+ *   bit 2  row offsets, those of padding entries included, that decrease, are negative or
+ *          pass the rows of the call
  *   bit 3  a slot past the cache, or a slot repeated in one write
  *   bit 4  a negative length, a length past the block table's row, or tokens read past it
  *   bit 5  a position past the rotary table

@@ -193,25 +193,26 @@ __device__ __forceinline__ void quantise_heads(const KittyKv8Cache& c, int slot,
 }
 
 // Entry i's slot, its rows [o, o + len) and the tokens it has; false for padding (a negative
-// slot), and (flagged) if any of them is out of range, or the slot is an earlier entry's.
+// slot), and (flagged) if any of them is out of range, or the slot is an earlier entry's.  The
+// offsets of padding are looked at too: rows are searched for among those of all entries.
 __device__ __forceinline__ bool entry_of(const KittyKv8WriteArgs& a, int i, bool first_cta, uint32_t* err, int& slot,
                                          int& o, int& len, int& cached) {
   uint32_t bad = 0;
   slot = a.seq_map ? a.seq_map[i] : i;
-  if (slot < 0) return false;
+  if (slot < 0 && !a.row_offsets) return false;
   o = a.row_offsets ? a.row_offsets[i] : i;
   const int64_t given = a.row_offsets ? int64_t(a.row_offsets[i + 1]) - o : 1;
   len = int(given);
   if (slot >= a.cache.slots) {
     bad = kErrSlot;
-  } else {
+  } else if (slot >= 0) {
     if (a.seq_map && dev::repeated(a.seq_map, i, slot)) bad = kErrSlot;
     cached = a.cache.lengths[slot];
     if (cached < 0 || cached > 0x7fffffff - a.rows) bad |= kErrLength;
   }
   if (o < 0 || given < 0 || o + given > a.rows) bad |= kErrRows;
   if (bad && first_cta && threadIdx.x == 0) dev::flag(err, bad);
-  return bad == 0;
+  return bad == 0 && slot >= 0;
 }
 
 __device__ __forceinline__ const uint16_t* row_of(const void* base, int64_t row, int64_t s_row, int64_t h, int64_t s_head) {

@@ -44,6 +44,7 @@ def write_kv8(key: torch.Tensor, value: torch.Tensor, lengths: torch.Tensor, blo
     before the next call on this cache (torch's indexing takes no negative slot; of single rows
     ``lengths.index_add_(0, seq_map.clamp(min=0), (seq_map >= 0).to(torch.int32))`` is safe with
     padding).  Rows behind the last offset are ignored.
+    The offsets of all entries, padding too, must not decrease.
     """
     _kv8.ops().write(key, value, lengths, block_table, key_codes, value_codes, key_scale, value_scale, tail_k, tail_v,
                      row_offsets, seq_map)

@@ -8,6 +8,7 @@ import torch
 
 from kitty import kernels as K
 from kv8_model import CacheModel
+from kv8_model import CacheModel
 from test_gpu_kv8 import E4M3, FP16, INT8, check_cache, filled, i32
 
 pytestmark = pytest.mark.gpu
@@ -62,3 +63,25 @@ def test_read_offsets_of_many_entries(n):
         bad[-1] = 3 * n + 1
         flags, k = read(m, bad, 3 * n, slots)
         assert flags == ROWS and torch.equal(k, want)
+
+
+def test_write_offsets_of_padding_entries():
+    """A write looks rows up by all entries' offsets, so those of padding have to follow one another
+    too: flagged where they do not, and padding that keeps the order is skipped silently."""
+    def fresh():
+        m = CacheModel(3, 2, 64, 32, E4M3, FP16, pages=8, table_width=4, seed=2)
+        return m, m.new_rows(69), m.new_rows(69)
+
+    for offsets, slots in (([0, 5, 69, 0, 0], [0, 2, -1, -1]), ([0, 5, 69, 69, 70], [0, 2, -1, -1]),
+                           ([-1, 0, 5, 69, 69], [-1, 0, 2, -1])):
+        m, k, v = fresh()
+        table = torch.arange(12, dtype=torch.int32).view(3, 4) % 8
+        K.write_kv8(k.cuda(), v.cuda(), m.lens(), *m.arrays(table), row_offsets=i32(offsets), seq_map=i32(slots))
+        assert K.kv8_error_flags() == ROWS, offsets
+    m, k, v = fresh()
+    before = m.lens()
+    m.append(0, k[:5], v[:5])
+    m.append(2, k[5:65], v[5:65])
+    K.write_kv8(k.cuda(), v.cuda(), before, *m.arrays(), row_offsets=i32([0, 5, 65, 69, 69]), seq_map=i32([0, 2, -1, -9]))
+    assert K.kv8_error_flags() == 0
+    check_cache(m)
