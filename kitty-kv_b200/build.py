@@ -18,6 +18,7 @@ import subprocess
 import sys
 import sysconfig
 from concurrent.futures import ThreadPoolExecutor
+from importlib import metadata
 from pathlib import Path
 
 PKG_ROOT = Path(__file__).resolve().parent
@@ -74,10 +75,24 @@ def _library(lib: Path, sources, headers, flags: list, verbose: bool, extra: lis
         subprocess.run(cmd, check=True)
         os.replace(tmp, lib)
 
+
+def _torch_built_for() -> str:
+    """What a module built against torch's C++ interface holds for."""
+    try:
+        torch_version = metadata.version("torch")
+    except metadata.PackageNotFoundError:
+        import torch
+        torch_version = torch.__version__
+    return f"torch {torch_version}, python {sys.version}\n"
+
+
 def _torch_module(module: Path, src: Path, lib: Path, verbose: bool) -> None:
-    """The Python extension module: the host compiler, torch's headers and libraries."""
+    """The Python extension module: the host compiler, torch's headers and libraries.  Built again
+    for another torch or Python too, whose C++ interface may differ."""
     header = REPO_ROOT / "include" / "kitty_kv8.h"
-    if module.exists() and module.stat().st_mtime >= max(src.stat().st_mtime, header.stat().st_mtime):
+    note, built_for = BUILD / (module.stem + ".txt"), _torch_built_for()
+    if (module.exists() and module.stat().st_mtime >= max(src.stat().st_mtime, header.stat().st_mtime)
+            and note.exists() and note.read_text() == built_for):
         return
     import torch
     root = Path(torch.__file__).resolve().parent
@@ -93,6 +108,7 @@ def _torch_module(module: Path, src: Path, lib: Path, verbose: bool) -> None:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
     os.replace(tmp, module)
+    note.write_text(built_for)
 
 
 if __name__ == "__main__":
