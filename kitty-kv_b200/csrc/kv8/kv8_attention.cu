@@ -219,73 +219,39 @@ struct Place {
   int64_t begin;       // first unit of the segment found
   int b, seg;          // its batch row and its index among the row's segments
 };
-// The same for at most kFew rows, by every warp for itself: no barrier, no second look at the
-// lengths, and all its loads at once.  Lane t has rows [t each, (t + 1) each).  256 sequences of up
-// to 60 tokens take 14.0 us so, 15.3 by the whole CTA.
-constexpr int kFewEach = 8, kFew = 32 * kFewEach;
+// The same for at most kFew rows, by every warp for itself: no barrier and no second look at the
+// lengths.  Lane t has row t.  8 sequences of up to 60 tokens take 8.7 us so and 8.9 by the whole
+// CTA, 32 take 9.5 and 9.7; with several rows a lane it is the slower one (64 sequences 11.6 and
+// 11.3, 256 of up to 8192 57.2 and 56.7).
+constexpr int kFew = 32;
 struct FewRows {
-  int one[kFewEach];                   // units of each row's segments
-  int64_t mine, before;                // of this lane's rows, and of the rows before them
+  int one;                             // units of each segment of the row
+  int64_t before;                      // units of one segment of each of the rows before it
 };
-// Returns the units of all rows (one segment of each).  kEach: 1 for at most 32 rows (a
-// call of one sequence takes 10.7 us, with room for 8 rows a lane 11.4), or kFewEach.
-template <int kTile, int kEach>
-__device__ __forceinline__ int64_t scan_few(const KittyKv8AttentionArgs& a, const Plan& plan, int per_row, int each,
-                                            FewRows& r, uint32_t* err) {
-  const int lane = threadIdx.x & 31, b0 = lane * each;
-  int slot[kEach], len[kEach];
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) slot[i] = i < each && b0 + i < a.batch ? (a.seq_map ? a.seq_map[b0 + i] : b0 + i) : -1;
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) len[i] = slot[i] >= 0 && slot[i] < a.cache.slots ? a.cache.lengths[slot[i]] : 0;
-  r.mine = 0;
-  uint32_t bad = 0;
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    if (slot[i] >= a.cache.slots) bad |= kErrSlot;
-    if (len[i] < 0 || blocks_of(plan, len[i]) > a.cache.max_pages) {
-      len[i] = 0;
-      bad |= kErrLength;
-    }
-    r.one[i] = tiles_of<kTile>(a.cache, plan, len[i]).units();
-    r.mine += r.one[i];
-  }
-  if (blockIdx.x == 0 && threadIdx.x < 32) {
-    if (bad) dev::flag(err, bad);
-    for (int i = 0; i < kEach; ++i)
-      if (i < each && b0 + i < a.batch && r.one[i] == 0)
-        for (int k = 0; k < per_row; ++k) plan.notes[int64_t(b0 + i) * per_row + k].units = 0;
-  }
-  int64_t incl = r.mine;
+// Returns the units of all rows (one segment of each).
+template <int kTile>
+__device__ __forceinline__ int64_t scan_few(const KittyKv8AttentionArgs& a, const Plan& plan, int per_row, FewRows& r,
+                                            uint32_t* err) {
+  const int b = threadIdx.x & 31;
+  r.one = units_of_row<kTile>(a, plan, b, blockIdx.x == 0 && threadIdx.x < 32 ? err : nullptr);
+  if (blockIdx.x == 0 && threadIdx.x < 32 && r.one == 0 && b < a.batch)
+    for (int k = 0; k < per_row; ++k) plan.notes[int64_t(b) * per_row + k].units = 0;
+  int64_t incl = r.one;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
+    if (b >= o) incl += v;
   }
-  r.before = incl - r.mine;
+  r.before = incl - r.one;
   return __shfl_sync(0xffffffffu, incl, 31);
 }
-template <int kEach>
-__device__ __forceinline__ Place locate_few(int per_row, int each, const FewRows& r, int64_t f) {
+__device__ __forceinline__ Place locate_few(int per_row, const FewRows& r, int64_t f) {
   int64_t at = r.before * per_row;
-  const uint32_t hit = __ballot_sync(0xffffffffu, f >= at && f < at + r.mine * per_row);
-  int len = 1, b = (threadIdx.x & 31) * each;
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {               // this lane's row that holds f, if it has it
-    const int64_t next = at + int64_t(r.one[i]) * per_row;
-    if (f >= next) {
-      at = next;
-      ++b;
-    } else if (f >= at) {
-      len = r.one[i];
-      break;
-    }
-  }
-  const int src = __ffs(hit) - 1;
+  const uint32_t hit = __ballot_sync(0xffffffffu, f >= at && f < at + int64_t(r.one) * per_row);
+  const int src = __ffs(hit) - 1, len = __shfl_sync(0xffffffffu, r.one, src);
   at = __shfl_sync(0xffffffffu, at, src);
-  len = __shfl_sync(0xffffffffu, len, src);
   const int seg = int(quotient(f - at, len));
-  return Place{at + int64_t(seg) * len, __shfl_sync(0xffffffffu, b, src), seg};
+  return Place{at + int64_t(seg) * len, src, seg};
 }
 
 // By the whole warp: the segment that holds unit f (less than there are).
@@ -370,18 +336,15 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
   // this warp's slice [f, f_end)
   __shared__ Rows s_rows;
   const bool few = a.batch <= kFew;
-  const int row_threads = few ? 32 : kWarps * 32, rows_each = (a.batch + row_threads - 1) / row_threads;
+  const int rows_each = (a.batch + kWarps * 32 - 1) / (kWarps * 32);
   FewRows few_rows;
-  const int64_t total = (rows_each == 1 && few ? scan_few<kTile, 1>(a, plan, per_row, 1, few_rows, err)
-                         : few ? scan_few<kTile, kFewEach>(a, plan, per_row, rows_each, few_rows, err)
-                               : scan_rows<kTile>(a, plan, per_row, rows_each, s_rows, err)) * per_row;
+  const int64_t total = (few ? scan_few<kTile>(a, plan, per_row, few_rows, err)
+                             : scan_rows<kTile>(a, plan, per_row, rows_each, s_rows, err)) * per_row;
   const int64_t per_warp = quotient(total + plan.warps - 1, plan.warps);
   const int64_t f0 = warp * per_warp, f_end = min(total, f0 + per_warp);
   if (f0 >= f_end) return;
   if (warp == 0 && lane == 0) plan.notes[int64_t(a.batch) * per_row].units = per_warp;
-  const Place at = rows_each == 1 && few ? locate_few<1>(per_row, 1, few_rows, f0)
-                   : few ? locate_few<kFewEach>(per_row, rows_each, few_rows, f0)
-                         : locate<kTile>(a, plan, per_row, rows_each, s_rows, f0);
+  const Place at = few ? locate_few(per_row, few_rows, f0) : locate<kTile>(a, plan, per_row, rows_each, s_rows, f0);
   int b = at.b, seg = at.seg;
   int64_t begin = at.begin;
 
