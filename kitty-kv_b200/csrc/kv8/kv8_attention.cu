@@ -27,8 +27,9 @@
 // keeps elements down to 2^-29 of it exact.  A weight is the sum of fp16 parts, two of 11 bits:
 // off by at most 2^-22 of itself or 2^-31 of the one at the reference (bf16 tails: three
 // parts of 8 bits).  With one part, 2^-12, the bf16 outputs over 32 x 32K tokens are 6e-4
-// (root mean square) from those of float32 weights, so 6e-5; that second part costs 3 % there
-// (337 against 326 us), 15 % with 16 query heads on a KV head (254 against 222).
+// (root mean square) from those of float32 weights, so 6e-5.  The second part costs 1 % there in
+// a burst (329 us against 326) and 8 % at the clocks of the power cap (380 against 352), with 16
+// query heads on a KV head 18 % (462 against 390).
 //
 // All segments' tiles (kTile tokens of a page, half as many of a tail: about the same
 // bytes) are laid end to end, each segment's behind kSetup units that stand for what a
@@ -222,7 +223,7 @@ struct Place {
 // The same for at most kFew rows, by every warp for itself: no barrier and no second look at the
 // lengths.  Lane t has row t.  8 sequences of up to 60 tokens take 8.7 us so and 8.9 by the whole
 // CTA, 32 take 9.5 and 9.7; with several rows a lane it is the slower one (64 sequences 11.6 and
-// 11.3, 256 of up to 8192 57.2 and 56.7).
+// 11.3, 256 of up to 8192 tokens 57.2 and 56.7).
 constexpr int kFew = 32;
 struct FewRows {
   int one;                             // units of each segment of the row
@@ -298,8 +299,9 @@ __device__ __forceinline__ bool cta_inside(int64_t cta, int64_t per_warp, int64_
 }
 
 // Warps hide one another's latency, so the registers are capped for 12 warps an SM at 128
-// channels (8 without a cap: 345 against 330 us for 32 x 32K tokens) and 16 at 64 (88 us for
-// the mixed batch at 12, 80 at 16, 81 at 20).
+// channels (32 x 32K tokens take 325 us, 341 with 8 warps and 432 with 16, 16 x 131K 664, 750 and
+// 826) and 16 at 64 (256 mixed lengths 57 us, 62 with 12 warps and 65 with 20).  Under the
+// cap up to 156 bytes a thread are spilled at 128 channels.
 template <int kDim>
 constexpr int kMinCtas = kDim == 64 ? 4 : kDim == 128 ? 3 : 1;
 
@@ -388,12 +390,12 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? kMinCtas<kDim> : 1)
         page = 0;
       }
     };
-    // Ask L2 for the page's next tiles, where it has at least kAhead of them: the loads of a
-    // tile find the following ones on their way.  Two tiles a page gain nothing by it (330
-    // against 330 us for 32 x 32K tokens at G = 64), four do (737 -> 686 us for 16 x 131K at
-    // G = 128); asking for more than 16 KB a warp costs (344 us at G = 64 for 32 KB).
+    // Ask L2 for the page's next tiles, where it has more than one: the loads of a tile find the
+    // following ones on their way.  32 x 32K tokens at G = 64 (two tiles) take 325 us with it and
+    // 332 without, 16 x 131K at G = 128 (four) 664 and 707; asking for eight at once costs (G =
+    // 256: 370 us, 327 with four), and so does asking for short sequences (8 x 8K: 35.2, 33.5).
     auto prefetch = [&]() {
-      if (per_block >= kAhead && sub % kAhead == 0 && lane < 2) {
+      if (per_block > 1 && sub % kAhead == 0 && lane < 2) {
         const int64_t at = ((int64_t(page) * H + h) * G + sub * kTile) * D;
         asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;"
                      :: "l"(static_cast<const uint8_t*>(lane ? c.value_codes : c.key_codes) + at),
@@ -860,7 +862,10 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(KittyKv8AttentionA
   const int heads = min(min(plan.pass_heads, g - q0) - first, heads_each);
   Note note{0, -2};
   int64_t per_warp = 1;
-  if (kTeam != 32 && a.batch <= 64) {                  // where the segment begins, while attention_kernel still runs
+  // Where the segment begins, while attention_kernel still runs: one sequence of 4096 tokens takes
+  // 9.3 us so and 9.9 with the note, 48 segments 18.3 and 18.8.  (Up to two rows a lane, which is
+  // all that segments for CTAs come to at 128 and 256 channels.)
+  if (kTeam != 32 && a.batch <= 64) {
     int64_t before = 0, total = 0;
     for (int i = threadIdx.x & 31; i < a.batch; i += 32) {
       const int64_t n = units_of_row<kTile, true>(a, plan, i);
@@ -1018,9 +1023,12 @@ int launch(const KittyKv8AttentionArgs& a, Plan plan, uint32_t* err, cudaStream_
   const int rc = launch_dependent("kv8_attention", attention_kernel<kDim, kNT, kWhole, kBf16, kCode>, dim3(unsigned(grid)),
                                   kWarps * 32, 0, s, a, plan, err);
   if (rc != KITTY_OK) return rc;
-  // Many warps to a segment: a CTA joins a head.  Otherwise a warp joins as many heads as it has
-  // lanes for: of 256 mixed lengths, 2048 segments of 5 heads, in 58.5 us all told (one head a
-  // warp 60.5, all five 60.8).
+  // Many warps to a segment: a CTA joins a head (128 channels, 8192 tokens each: 48 segments take
+  // 25.9 us so and 29.8 with warps).  The two meet at 76 segments whatever the channels, which is
+  // where the rule changes at 64; at 128 channels 56 to 72 segments, and at 256 from 40 on, would
+  // still be 2 to 7 us faster with CTAs.  Otherwise a warp joins as many heads as it has lanes
+  // for: 256 mixed lengths, 2048 segments of 5 heads, take 57.0 us all told (one head a warp
+  // 58.8, all five 59.2).
   const int64_t segments = int64_t(a.batch) * a.cache.num_heads * plan.passes;
   const int heads_each = std::min(std::max(1, 128 / a.cache.head_dim), plan.pass_heads);
   return segments * 32 < plan.warps ? launch_merge<kTileOf<kDim>, kBf16, kMergeThreads>(a, plan, 1, s)
