@@ -1,5 +1,8 @@
 // Shared pieces of the 8-bit cache kernels: the host-side checks, the sticky device
 // error bits and the conversions between 16-bit rows, 8-bit codes and float32.
+//
+// Times in these files are of calls replayed from a CUDA graph in a burst on one B200 at full
+// clocks, over three caches, unless they say otherwise.
 #pragma once
 
 #include <cuda_bf16.h>

@@ -4,7 +4,7 @@
 // and page and leaves them in shared memory: 32 entries' offsets, slots and first tokens are
 // loaded at once and searched by shuffles, then the row's page and its slot's length, also at
 // once.  (A search in memory is a chain of loads, 5 for 24 entries: 24 ragged chunks are
-// written and read in 17.3 us so, 17.8 with it; one entry of 4137 tokens in 9.1 and 8.7.  With
+// written and read in 16.4 us so, 16.8 with it; one entry of 4137 tokens in 8.9 and 8.5.  With
 // the length first and the page behind it, 16 x 32768 tokens took 576 us instead of 507.)
 // Then every thread turns eight codes of keys and of values (8 bytes each) into 16-byte
 // stores, contiguous over the row, at the same place of one row after another.  Bound by
@@ -146,7 +146,10 @@ __global__ void __launch_bounds__(kThreads) read_kernel(KittyKv8ReadArgs a, uint
 
 template <bool kBf16, int kCode>
 int launch(const KittyKv8ReadArgs& a, uint32_t* err, cudaStream_t s) {
-  // Many rows: 32 a CTA, which finds their pages once.  Few: 8, so that every SM has some.
+  // Many rows: 32 a CTA, which finds their pages once (16 x 32768 tokens of 8 heads of 128: 505 us
+  // in a burst and 509 at the clocks of the power cap, with 8 rows 499 and 531; of one head 174,
+  // with 8 rows 446).  Few: 8, so that every SM has some (one entry of 4137 tokens 8.9 us, 15.4
+  // with 32).
   if (int64_t(a.rows) * a.cache.num_heads * a.cache.head_dim > kManyValues * sm_count())
     return launch_dependent("kv8_read", read_kernel<kBf16, kCode, 32>, dim3(unsigned((int64_t(a.rows) + 31) / 32)),
                             kThreads, 0, s, a, err);

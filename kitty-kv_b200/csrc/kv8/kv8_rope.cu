@@ -203,9 +203,9 @@ int launch(const KittyQkNormRopeArgs& a, uint32_t* err, cudaStream_t s) {
 
 template <bool kBf16, int kLanes>
 int launch_size(const KittyQkNormRopeArgs& a, uint32_t* err, cudaStream_t s) {
-  // Stages pay where a resident warp has more than one token (40 heads of 128: 8.0 against
-  // 9.3 us for 1024 tokens, 32 against 40 for 8192, 114 against 119 for 32768) and cost where it
-  // has one (301 tokens of 72 heads: 6.3 and 5.1 us).
+  // Stages pay where a resident warp has more than one token (40 heads of 128: 6.1 against
+  // 6.4 us for 1024 tokens, 31 against 38 for 8192, 111 against 136 for 32768) and cost where it
+  // has one (301 tokens of 72 heads: 5.6 and 4.6 us).
   // With no more heads than a warp has lane groups, rows behind the first would be empty.
   if (std::max(a.num_q_heads, a.num_k_heads) <= 32 / kLanes) return launch<kBf16, kLanes, 1, 0>(a, err, s);
   constexpr int kStaged = 4, kHeads = 32 / kLanes * kStaged;

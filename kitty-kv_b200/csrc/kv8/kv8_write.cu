@@ -11,8 +11,10 @@
 //
 // A block of one head (G x D values) is read once into registers where it fits, its
 // largest magnitude taken with packed 16-bit maxima (exact), and the codes stored from
-// registers: 2 bytes read and 1 written a value, the floor of this operation.  Of small
-// blocks a CTA takes several heads, so that its threads have as much to do.
+// registers: 2 bytes read and 1 written a value, the floor of this operation.  (With one head a
+// CTA, where each place of a block stands three times in the code, 64 registers do not hold all
+// of it: 88 bytes a thread are spilled.)  Of small blocks a CTA takes several heads, so that its
+// threads have as much to do.
 #include "kv8_common.cuh"
 
 namespace kitty8 {
@@ -20,7 +22,7 @@ namespace {
 
 constexpr int kHeld = 4;        // 16-byte vectors a thread holds in registers for each of key and value
 constexpr int kThreads = 256;
-constexpr int kMinCtas = 4;     // resident on an SM: 78K ragged rows take 109 us at 2, 88 at 3, 77 at 4, 96 at 5
+constexpr int kMinCtas = 4;     // resident on an SM: 75K ragged rows take 108 us at 2, 86 at 3, 76 at 4, 95 at 5
 constexpr int kStepEntries = 8; // entries of a decode step whose blocks one CTA looks after
 
 // Source rows of a block: the first `have` from the tail, the others from the call's rows.
@@ -126,7 +128,8 @@ __device__ __forceinline__ void quantise_rows(const KittyKv8Cache& c, int slot, 
 
 // Keys and values together where they fit the registers.  A larger block is read twice, the
 // second time from L2, and one kind after the other keeps what is in use small enough for it
-// (28K tokens, 4 heads of 256, 256-token pages: 129 against 147 us; 8 of 128: 41 against 45).
+// (29K tokens, 4 heads of 256, 256-token pages: 46 us, both kinds together 63; 8 of 128: 40 and
+// 44; 75K tokens of 8 of 128 in 128-token pages: 86 and 84).
 template <bool kBf16, int kCode, int kPer>
 __device__ __forceinline__ void quantise_block(const KittyKv8Cache& c, int slot, int block, int h, const Rows (&src)[2],
                                                uint32_t (*s_top)[kThreads / 32], uint32_t* err) {
@@ -143,7 +146,7 @@ __device__ __forceinline__ void quantise_block(const KittyKv8Cache& c, int slot,
 
 // The same for a block's heads h .. h + heads - 1 (at most 2^shift), 2^-shift of the CTA's warps
 // for each, whose registers hold it.  kShift: the shift, known when compiled (75K ragged rows of
-// 8 heads of 128 in 32-token pages: 75 us, 85 otherwise), or -1.
+// 8 heads of 128 in 32-token pages: 74 us, 84 otherwise), or -1.
 template <bool kBf16, int kCode, int kPer, int kShift>
 __device__ __forceinline__ void quantise_heads(const KittyKv8Cache& c, int slot, int block, int h, int heads, int shift_,
                                                const Rows (&src)[2], const int64_t (&s_head)[2],
@@ -336,8 +339,8 @@ int launch(const KittyKv8WriteArgs& a, uint32_t* err, cudaStream_t s) {
   const int64_t H = a.cache.num_heads, items = int64_t(a.n) + a.rows / a.cache.page_size;
   const int64_t steps = (int64_t(a.n) + kStepEntries - 1) / kStepEntries * H + a.n;
   // Heads of a CTA: as many as its registers hold, unless fewer than the card's CTAs are left
-  // to share the work.  75K ragged rows of 8 heads of 64 in 32-token pages take 40.5 us, with one
-  // head each 115; 300 rows 4.1, with four heads each 5.4.
+  // to share the work.  75K ragged rows of 8 heads of 64 in 32-token pages take 39 us, with one
+  // head each 113; 300 rows 3.0, with four heads each 4.0.
   const int vecs = a.cache.page_size * a.cache.head_dim / 8;
   int shift = 0;
   const auto ctas = [&] { return items * ((H + (1 << shift) - 1) >> shift); };
