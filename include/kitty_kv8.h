@@ -88,10 +88,10 @@ typedef struct KittyKv8Cache {
  * key / value (row r, head h, channel c at base + r*s_row + h*s_head + c; 16-byte
  * aligned rows) behind the lengths[slot] tokens that it has, slot = seq_map[i] (NULL:
  * i).  row_offsets NULL: one row each, n == rows.  Rows behind the last offset are
- * ignored, and so are entries of a negative slot (padding).  Blocks that fill are quantised into their pages, which block_table must
- * hold; the rest goes to the tail.  `lengths` is not changed: the caller adds the new
- * tokens before it reads the cache.  One launch.  A slot given twice keeps its first
- * entry. */
+ * ignored, and so are entries of a negative slot (padding).  Blocks that fill are
+ * quantised into their pages, which block_table must hold; the rest goes to the tail.
+ * `lengths` is not changed: the caller adds the new tokens before it reads the cache.
+ * One launch.  A slot given twice keeps its first entry. */
 typedef struct KittyKv8WriteArgs {
   KittyKv8Cache cache;
   const void* key;
@@ -123,11 +123,12 @@ int kitty_kv8_read(const KittyKv8ReadArgs* args, void* stream);
 
 /* Decode attention: out[b][qh] = softmax(sm_scale * q[b][qh] . k) . v over the
  * lengths[slot] tokens of slot seq_map[b] (NULL: b), KV head qh / (Hq / H); zeros for
- * an empty slot and for a negative one (padding).  q and out have the cache's 16-bit type; sums and softmax statistics
- * are float32; the weights that multiply the values are off by at most 2^-22 of
- * themselves, or 2^-31 of the largest.  bf16 values may be as large as 2^128 / tokens
- * (a float32 sum of weights of at most 1).  The workspace (16-byte aligned) holds the partial results of
- * sequences that several warps share; calls that overlap must not share one. */
+ * an empty slot and for a negative one (padding).  q and out have the cache's 16-bit
+ * type (out may be q itself, with the same strides); sums and softmax statistics are
+ * float32; the weights that multiply the values are off by at most 2^-22 of themselves,
+ * or 2^-31 of the largest.  bf16 values may be as large as 2^128 / tokens (a float32 sum
+ * of weights of at most 1).  The workspace (16-byte aligned) holds the partial results
+ * of sequences that several warps share; calls that overlap must not share one. */
 typedef struct KittyKv8AttentionArgs {
   KittyKv8Cache cache;
   const void* q;

@@ -301,7 +301,7 @@ __device__ __forceinline__ bool cta_inside(int64_t cta, int64_t per_warp, int64_
 // Warps hide one another's latency, so the registers are capped for 12 warps an SM at 128
 // channels (32 x 32K tokens take 325 us, 341 with 8 warps and 432 with 16, 16 x 131K 664, 750 and
 // 826) and 16 at 64 (256 mixed lengths 57 us, 62 with 12 warps and 65 with 20).  Under the
-// cap up to 156 bytes a thread are spilled at 128 channels.
+// cap 80 to 104 bytes a thread are spilled at 128 channels.
 template <int kDim>
 constexpr int kMinCtas = kDim == 64 ? 4 : kDim == 128 ? 3 : 1;
 

@@ -41,8 +41,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
     position; float16 or bfloat16, float32 inside, rounded once.  Returns (q_out, k_out).
 
     positions: (N,) int32 or int64 rows of ``table`` (:func:`rope_table`); a negative
-    position marks a padding row, whose output is left as it was; one past the table
-    does the same and sets a sticky error bit (:func:`kv8_error_flags`).
+    position marks a padding row, whose output is left as it was (undefined where the
+    output is made here); one past the table does the same and sets a sticky error bit
+    (:func:`kv8_error_flags`).
     table: (max_positions, R) float32; channels from R on are normalised only.
     q_weight / k_weight: (D,) of q's dtype or float32, both or neither; without them
     there is no norm, only the rotation.
