@@ -61,7 +61,8 @@ def read_kv8(lengths: torch.Tensor, block_table: torch.Tensor, key_codes: torch.
     ``seq_map[i]`` (without it i) from ``first[i]`` (without it 0) on.  Rows behind the
     last offset, of a negative slot, and of tokens that the slot does not have are left as they
     were (``key_out`` / ``value_out``: the caller's tensors, contiguous, not overlapping; undefined
-    in tensors made here).
+    in tensors made here).  The offsets of all entries, padding too, must not decrease or pass
+    ``rows``.
     """
     return _kv8.ops().read(lengths, block_table, key_codes, value_codes, key_scale, value_scale, tail_k, tail_v,
                            row_offsets, rows, first, seq_map, key_out, value_out)
