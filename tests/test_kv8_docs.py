@@ -13,8 +13,9 @@ ROOT = Path(__file__).resolve().parent.parent
 
 
 def test_documented_advance_of_lengths_takes_padding():
-    """Every documented line that adds a step's tokens to the lengths, with padded slots."""
-    texts = [p.read_text() for p in ROOT.glob("*.md")] + [K.write_kv8.__doc__]
+    """The lines of the integration document and of the docstring that add a step's tokens to the
+    lengths, with padded slots."""
+    texts = [p.read_text() for p in ROOT.glob("INTEGR*")] + [K.write_kv8.__doc__]
     lines = [x for t in texts for x in re.findall(r"lengths\.index_add_\(.*\)", t)]
     assert len(lines) >= 2
     for line in lines:
